@@ -19,6 +19,9 @@ FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # every elementwise op rounds like the reference's unfused ATen ops; FMAs are explicit
     "-ffp-contract=off",
+    # no packed-f32 instructions (v_pk_fma_f32 and its like): some of their forms have given wrong
+    # values now and then on this hardware.  The host pass warns that it does not know the feature.
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
 

@@ -1078,8 +1078,8 @@ __device__ __forceinline__ float gather_certainty(const Src& src, const Neighbou
 
 // Decoder weights staged in LDS once per block (stage_mlp), laid out for the packed loop:
 // hidden units in pairs (c, c+1), W1 interleaved per input i as {W1[c][i], W1[c+1][i]}
-// (12 inputs incl. one pad -> 24 floats per pair), then b1, W2, b2.  A pair's operand for
-// v_pk_fma_f32 is one 8-B broadcast LDS read; broadcast reads return in order, so several
+// (12 inputs incl. one pad -> 24 floats per pair), then b1, W2, b2.  A pair's operand is one
+// 8-B broadcast LDS read (two scalar FMAs: the build takes no packed-f32 instructions); broadcast reads return in order, so several
 // stay in flight (the scalar-load form paid a dependent K$ round trip per pair).
 constexpr int kWRow = 12;                    // padded inputs per hidden unit
 constexpr int kWPair = 2 * kWRow;            // floats per hidden-unit pair
@@ -1142,7 +1142,7 @@ __device__ __forceinline__ void load_row(const float* __restrict__ w, int c, flo
 
 // Decoder forward fused with its input gradient (model/decoder.py:66-88):
 //   sdf = s * (w2 . relu(W1 x + b1) + b2),  gx[i] = s * sum_c w2[c] 1[pre_c > 0] W1[c][OFF+i].
-// One pass over the hidden units, two at a time with packed FMAs (v_pk_fma_f32).
+// One pass over the hidden units, two at a time (one 8-B weight read, two scalar FMAs).
 // mask (may be NULL): the 64 ReLU masks, bit c = [pre_c > 0] (the per-neighbour training forward
 // saves them for the backward's input gradient, mlp_grad8_from_mask).
 template <bool GRAD, int OFF, int NOUT>
