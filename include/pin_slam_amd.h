@@ -937,6 +937,77 @@ int pin_mc_count(const float* values, const uint8_t* mask, int64_t nx, int64_t n
 int pin_mc_emit(const float* values, int64_t nx, int64_t ny, int64_t nz, float level, const void* workspace,
                 float* verts, int32_t* faces, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Training with class labels: the loss beside Decoder.sem_label_prob (model/decoder.py:120)
+ * and an optimiser step over many tensors.  Tensors may be f32 or 16 bits wide. */
+#define PIN_TYPE_F32 0
+#define PIN_TYPE_F16 1
+#define PIN_TYPE_BF16 2
+
+#define PIN_LABEL_TOP_MAX 32             /* most alternatives per row */
+#define PIN_LABEL_CLASSES_MAX 16777216   /* most classes (2^24) */
+
+/*
+ * pin_label_logprob -- for each of n rows of `classes` logits (type `dtype`, consecutive classes
+ * adjacent, rows row_stride elements apart) with p = softmax(row):
+ *   log_prob [n]        log p of the row's label, 0 where the label is ignore_index
+ *   entropy [n]         -sum p log p
+ *   row_stats [n,2]     the row's maximum and log sum exp(row - maximum) (for the gradient; may be NULL)
+ *   top_log_prob, top_index [n,top_k]   the top_k most probable classes, ties to the lower class
+ * Classes at -inf have no share.  All of a row at -inf: log_prob -inf, entropy 0, classes 0..top_k-1
+ * at -inf.  A NaN or +inf in a row: NaN, top_index -1.  A label outside [0, classes) that is not
+ * ignore_index: log_prob NaN.  workspace: pin_label_logprob_workspace_bytes bytes, 16-byte aligned
+ * (NULL where that is 0), free again when the call's work on the stream is done.
+ */
+int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dtype, int32_t top_k);
+int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
+                      const int64_t* labels, int64_t ignore_index, int32_t top_k, float* log_prob, float* entropy,
+                      float* row_stats, float* top_log_prob, int64_t* top_index, void* workspace, void* stream);
+
+/*
+ * pin_label_logprob_bwd -- d_logits [n, classes] (type `dtype`, contiguous) from the gradients of
+ * log_prob, entropy and top_log_prob (each may be NULL: zero), recomputing the probabilities from
+ * the logits and pin_label_logprob's row_stats, entropy and top_index.  An ignored label takes no
+ * part; a row without a distribution has gradient 0.
+ */
+int pin_label_logprob_bwd(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
+                          const int64_t* labels, int64_t ignore_index, int32_t top_k, const int64_t* top_index,
+                          const float* row_stats, const float* entropy, const float* d_log_prob,
+                          const float* d_entropy, const float* d_top, void* d_logits, void* stream);
+
+#define PIN_ADAMW_BLOCK 256              /* elements that share the exponents of an 8-bit moment */
+#define PIN_ADAMW_SCALARS_BYTES 64
+
+/*
+ * pin_adamw_step -- one AdamW step over `count` tensors in place (host arrays of device pointers and
+ * sizes; parameters and gradients contiguous, of type `dtype`):
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * The state of tensor k lies at elements offsets[k] .. offsets[k] + sizes[k] of flat arrays of
+ * state_elements; offsets are multiples of PIN_ADAMW_BLOCK in rising order, the elements behind a
+ * tensor up to the next multiple are the array's own (and stay zero).  state_bits 32: exp_avg and
+ * exp_avg_sq are f32.  state_bits 8: uint8 codes, with exponents [state_elements / PIN_ADAMW_BLOCK, 2]
+ * int16 (pin_adamw.hip describes them); zero bytes stand for zero moments.  master (f32, may be NULL):
+ * the parameters' values in 32 bits, from which the step goes on; params then get their rounding.
+ * salt: seeds the 8-bit moments' rounding, which depends on it, the step and the element's place.
+ * scalars: NULL, or what pin_adamw_scalars wrote (lr, betas, weight_decay, step and salt are then not
+ * read): a step that a captured graph may replay.
+ */
+int pin_adamw_step(void* const* params, const void* const* grads, const int64_t* sizes, const int64_t* offsets,
+                   int32_t count, int32_t dtype, int32_t state_bits, void* exp_avg, void* exp_avg_sq,
+                   int16_t* exponents, float* master, int64_t state_elements, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, int64_t step, uint32_t salt, const void* scalars, void* stream);
+
+/* pin_adamw_scalars -- step (device) += 1, and the scalars of that step into `scalars`
+ * (PIN_ADAMW_SCALARS_BYTES, device, 8-byte aligned); lr_device (device, may be NULL) in lr's place. */
+int pin_adamw_scalars(int64_t* step, const float* lr_device, double lr, double beta1, double beta2,
+                      double weight_decay, uint32_t salt, void* scalars, void* stream);
+
+/* pin_adamw_moments -- the values that 8-bit moments stand for: n elements (a multiple of
+ * PIN_ADAMW_BLOCK) of both, as f32. */
+int pin_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const int16_t* exponents, int64_t n, float* m,
+                      float* v, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

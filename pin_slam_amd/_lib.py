@@ -3,6 +3,7 @@
 The library is REQUIRED: there is no CPU or eager-PyTorch fallback for the hot
 path.  If the shared object is missing or a call fails, this module raises.
 """
+import contextlib
 import ctypes
 import os
 
@@ -30,7 +31,9 @@ RECORD_UNFAITHFUL = 1 << 30
 c_void_p = ctypes.c_void_p
 i32 = ctypes.c_int32
 i64 = ctypes.c_int64
+u32 = ctypes.c_uint32
 f32 = ctypes.c_float
+f64 = ctypes.c_double
 
 
 class PinHash(ctypes.Structure):
@@ -116,6 +119,11 @@ class PinRowArray(ctypes.Structure):
 
 
 ROW_ARRAYS_MAX = 8   # PIN_ROW_ARRAYS_MAX
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # PIN_TYPE_*
+LABEL_TOP_MAX = 32             # PIN_LABEL_TOP_MAX
+LABEL_CLASSES_MAX = 1 << 24    # PIN_LABEL_CLASSES_MAX
+ADAMW_BLOCK = 256              # PIN_ADAMW_BLOCK
+ADAMW_SCALARS_BYTES = 64       # PIN_ADAMW_SCALARS_BYTES
 MLP_GRAD_FIRST, MLP_GRAD_SECOND = 1, 2   # pin_mlp_backward flags
 
 MLP_GRAD_SIZE = HIDDEN_DIM * (FEATURE_DIM + 3) + 2 * HIDDEN_DIM + 1
@@ -218,11 +226,20 @@ _SIGS = {
     "pin_map_gather": [_P(PinMapArrays), c_void_p, i64, i32, _P(PinMapArrays), c_void_p],
     "pin_map_scatter": [_P(PinMapArrays), c_void_p, i64, i32, _P(PinMapArrays), c_void_p],
     "pin_map_adjust": [_P(PinMapArrays), c_void_p, i64, i32, c_void_p],
+    "pin_label_logprob_workspace_bytes": [i64, i64, i32, i32],
+    "pin_label_logprob": [c_void_p, i32, i64, i64, i64, c_void_p, i64, i32, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_void_p, c_void_p, c_void_p],
+    "pin_label_logprob_bwd": [c_void_p, i32, i64, i64, i64, c_void_p, i64, i32, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_void_p],
+    "pin_adamw_step": [_P(c_void_p), _P(c_void_p), _P(i64), _P(i64), i32, i32, i32, c_void_p, c_void_p, c_void_p,
+                       c_void_p, i64, f64, f64, f64, f64, f64, i64, u32, c_void_p, c_void_p],
+    "pin_adamw_scalars": [c_void_p, c_void_p, f64, f64, f64, f64, u32, c_void_p, c_void_p],
+    "pin_adamw_moments": [c_void_p, c_void_p, c_void_p, i64, c_void_p, c_void_p, c_void_p],
 }
 # functions whose return value is not a status code
 _RESTYPES = {"pin_map_workspace_bytes": i64, "pin_mc_workspace_bytes": i64,
              "pin_query_sort_stable_workspace_bytes": i64, "pin_mlp_backward_workspace_bytes": i64,
-             "pin_pool_window_workspace_bytes": i64}
+             "pin_pool_window_workspace_bytes": i64, "pin_label_logprob_workspace_bytes": i64}
 
 _lib = None
 
@@ -298,6 +315,14 @@ def stream(device=None):
             idx = torch.cuda.current_device() if idx is None else idx
         return c_void_p(_raw_stream(idx))
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(device):
+    """Context in which launches go to ``device`` (nothing to do where it is the current one)."""
+    device = torch.device(device)
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_device(t):

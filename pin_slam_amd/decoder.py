@@ -18,6 +18,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .label_logprob import label_log_probs
 
 # PIN_DECODER_ATEN=1: Decoder.sdf through the nn.Linear layers (A/B and restatement checks)
 _ATEN_SDF = os.environ.get("PIN_DECODER_ATEN", "0") == "1"
@@ -169,6 +170,11 @@ class Decoder(nn.Module):
 
     def sem_label(self, features):
         return torch.argmax(self.sem_label_prob(features), dim=1)
+
+    def sem_label_log_prob(self, features, labels, top_k=0, ignore_index=-100):
+        """The log probabilities sem_label_prob gives to ``labels``, with each row's entropy and its
+        top_k most probable classes (label_log_probs of the head's logits, with their gradient)."""
+        return label_log_probs(self.lout(self._trunk(features)), labels, top_k, ignore_index)
 
     def regress_color(self, features):
         return torch.clamp(self.lout(self._trunk(features)), 0.0, 1.0)

@@ -1,0 +1,285 @@
+"""AdamW over many tensors at once, its moments held in 32 bits or in 8 (pin_adamw_step).
+
+The optimiser beside the mapping loop's own Adam launches, for what a program trains through
+autograd: heads, features and networks of any number of tensors in f32, f16 or bf16
+(utils/tools.py:89-116 builds the reference's torch.optim.Adam from the same kinds of groups, and
+its rates are the defaults here).  A step is one launch for up to 112 tensors of one group, type
+and step count.
+
+The state of a parameter group lies in flat arrays in which every parameter begins at a multiple
+of 256 elements (``offsets``); ``state[p]`` holds views of them.  With state_bits 8 a moment takes
+one byte per element and two bytes per 256, rounded so that its expectation is kept
+(csrc/pin_adamw.hip).
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+
+_SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
+_STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
+
+
+def _blocks(n):
+    return -(-n // _lib.ADAMW_BLOCK)
+
+
+class _Arena:
+    """The state of one parameter group."""
+
+    def __init__(self, group, capturable):
+        params = group["params"]
+        bits = group["state_bits"]
+        dev = params[0].device
+        self.bits, self.device = bits, dev
+        self.sizes = [p.numel() for p in params]
+        self.offsets, total = [], 0
+        for n in self.sizes:
+            self.offsets.append(total)
+            total += _blocks(n) * _lib.ADAMW_BLOCK
+        self.total = total
+        kind = torch.float32 if bits == 32 else torch.uint8
+        self.m = torch.zeros((total,), dtype=kind, device=dev)
+        self.v = torch.zeros((total,), dtype=kind, device=dev)
+        self.exps = torch.zeros((total // _lib.ADAMW_BLOCK, 2), dtype=torch.int16, device=dev) if bits == 8 else None
+        self.master = None
+        if group["master_weights"] and any(p.dtype != torch.float32 for p in params):
+            self.master = torch.zeros((total,), dtype=torch.float32, device=dev)
+            for p, a, n in zip(params, self.offsets, self.sizes):
+                self.master[a:a + n] = p.detach().reshape(-1)
+        self.steps = [0] * len(params)
+        # a step that a graph may replay counts on the device, all of the group's parameters together
+        self.step_dev = torch.zeros((1,), dtype=torch.int64, device=dev) if capturable else None
+        self.scalars = torch.zeros((_lib.ADAMW_SCALARS_BYTES,), dtype=torch.uint8, device=dev) if capturable else None
+
+    def views(self, i, shape):
+        """The parameter's part of each array."""
+        a, n = self.offsets[i], self.sizes[i]
+        one = {"exp_avg": self.m[a:a + n].view(shape), "exp_avg_sq": self.v[a:a + n].view(shape)}
+        if self.exps is not None:
+            one["exponents"] = self.exps[a // _lib.ADAMW_BLOCK:a // _lib.ADAMW_BLOCK + _blocks(n)]
+        if self.master is not None:
+            one["master"] = self.master[a:a + n].view(shape)
+        return one
+
+
+class AdamW(torch.optim.Optimizer):
+    """Parameters p with gradients g, per step t of the parameter:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    lr, betas, eps, weight_decay, state_bits (32 or 8) and master_weights (16-bit parameters keep a
+    copy in 32 bits that the steps go on from) may differ by parameter group; parameters of a group
+    share a device and are contiguous.  seed chooses the 8-bit moments' rounding.
+
+    capturable: step() may be captured into a graph after one eager step; a group's parameters then
+    all have gradients and count steps together, and lr may be a float32 tensor on the device that
+    replays read (a number is taken as it was when captured).
+
+    The state is made at the first step (or by load_state_dict); parameters are neither added to a
+    group, reshaped nor moved to another device afterwards."""
+
+    def __init__(self, params, lr=0.01, betas=(0.9, 0.99), eps=1e-15, weight_decay=0.0, *, state_bits=32,
+                 master_weights=False, capturable=False, seed=0):
+        self.capturable, self.seed = bool(capturable), int(seed)
+        self._arenas = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=bool(master_weights)))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _check_group(self, group):
+        lr, (b1, b2) = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor):
+            if not self.capturable or lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("AdamW: a tensor lr must be one float32 on the device, with capturable=True")
+        elif not 0.0 <= lr < float("inf"):
+            raise ValueError(f"AdamW: lr must be >= 0 (got {lr})")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1) (got {group['betas']})")
+        if not 0.0 <= group["eps"] < float("inf") or not 0.0 <= group["weight_decay"] < float("inf"):
+            raise ValueError(f"AdamW: eps and weight_decay must be >= 0 (got {group['eps']}, {group['weight_decay']})")
+        if group["state_bits"] not in _STATE_KEYS:
+            raise ValueError(f"AdamW: state_bits must be 32 or 8 (got {group['state_bits']})")
+        params = group["params"]
+        spans = []
+        for p in params:
+            if p.dtype not in _lib.TYPES:
+                raise ValueError(f"AdamW: parameters must be float32, float16 or bfloat16 (got {p.dtype})")
+            if p.layout != torch.strided or not p.is_contiguous():
+                raise ValueError("AdamW: parameters must be contiguous")
+            if p.device != params[0].device:
+                raise ValueError("AdamW: the parameters of a group must be on one device")
+            spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        for other in self.param_groups:
+            if other is not group:
+                spans += [(p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in other["params"]]
+        spans = sorted(s for s in spans if s[1] > s[0])
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters share memory")
+
+    def _arena(self, gi):
+        group = self.param_groups[gi]
+        arena = self._arenas.get(gi)
+        if arena is None:
+            for p in group["params"]:
+                _lib.require_device(p)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: run one step before capturing one (it makes the state)")
+            arena = self._arenas[gi] = _Arena(group, self.capturable)
+            for i, p in enumerate(group["params"]):
+                self.state[p] = arena.views(i, p.shape)
+        if len(arena.sizes) != len(group["params"]):
+            raise RuntimeError("AdamW: parameters were added to or taken from a group after its first step")
+        return arena
+
+    def _gather(self, arena, group):
+        """Indexes, parameters and gradients of what has a gradient, checked."""
+        todo = []
+        for i, p in enumerate(group["params"]):
+            g = p.grad
+            if g is None:
+                if self.capturable:
+                    raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
+                continue
+            if g.layout != torch.strided:
+                raise RuntimeError("AdamW: sparse gradients are not implemented")
+            if p.numel() != arena.sizes[i] or p.device != arena.device or not p.is_contiguous():
+                raise RuntimeError("AdamW: a parameter was reshaped or moved after its first step")
+            if g.dtype != p.dtype or g.device != arena.device or p.dtype not in _lib.TYPES:
+                raise RuntimeError(f"AdamW: a {p.dtype} parameter on {p.device} has a {g.dtype} gradient on {g.device}")
+            todo.append((i, p, g if g.is_contiguous() else g.contiguous()))
+        return todo
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for gi, group in enumerate(self.param_groups):   # everything is checked before anything is stepped
+            if not group["params"] or not (self.capturable or any(p.grad is not None for p in group["params"])):
+                continue
+            _lib.require_device(group["params"][0])
+            if not self.capturable and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: capturing a step needs capturable=True (the step count is on the host)")
+            arena = self._arena(gi)
+            work.append((gi, group, arena, self._gather(arena, group)))
+        for gi, group, arena, todo in work:
+            with _lib.on_device(arena.device):
+                self._step_group(gi, group, arena, todo)
+        return loss
+
+    def _salt(self, gi):
+        return (self.seed * _SALT_SEED + gi * _SALT_GROUP) & 0xFFFFFFFF
+
+    def _step_group(self, gi, group, arena, todo):
+        lr, (b1, b2) = group["lr"], group["betas"]
+        stream = _lib.stream(arena.device)
+        wd, salt = float(group["weight_decay"]), self._salt(gi)
+        lr_dev = lr if isinstance(lr, torch.Tensor) else None
+        rates = (0.0 if lr_dev is not None else float(lr), float(b1), float(b2))
+        if self.capturable:
+            _lib.call("pin_adamw_scalars", _lib.ptr(arena.step_dev), _lib.ptr(lr_dev), *rates, wd, salt,
+                      _lib.ptr(arena.scalars), stream)
+        buckets = {}
+        for i, p, g in todo:
+            if not self.capturable:
+                arena.steps[i] += 1
+            buckets.setdefault((p.dtype, arena.steps[i]), []).append((i, p, g))
+        for (dtype, t), some in buckets.items():
+            n = len(some)
+            ps = (ctypes.c_void_p * n)(*[p.data_ptr() for _, p, _ in some])
+            gs = (ctypes.c_void_p * n)(*[g.data_ptr() for _, _, g in some])
+            sizes = (ctypes.c_int64 * n)(*[arena.sizes[i] for i, _, _ in some])
+            offsets = (ctypes.c_int64 * n)(*[arena.offsets[i] for i, _, _ in some])
+            master = arena.master if dtype != torch.float32 else None
+            _lib.call("pin_adamw_step", ps, gs, sizes, offsets, n, _lib.TYPES[dtype], arena.bits, _lib.ptr(arena.m),
+                      _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total, *rates,
+                      float(group["eps"]), wd, t, salt, _lib.ptr(arena.scalars), stream)
+
+    def offsets(self, group=0):
+        """First element of each parameter of the group in the flat arrays."""
+        return list(self._arena(group).offsets)
+
+    def moments(self, group=0):
+        """Both moments of a parameter group as flat float32 arrays (of 8-bit state: the values that
+        its codes stand for; of 32-bit state: the state itself)."""
+        arena = self._arena(group)
+        if arena.bits == 32:
+            return arena.m, arena.v
+        m = torch.empty((arena.total,), dtype=torch.float32, device=arena.device)
+        v = torch.empty_like(m)
+        with _lib.on_device(arena.device):
+            _lib.call("pin_adamw_moments", _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), arena.total,
+                      _lib.ptr(m), _lib.ptr(v), _lib.stream(arena.device))
+        return m, v
+
+    def master(self, group=0):
+        """The group's parameters in 32 bits as one flat array (None without master_weights)."""
+        return self._arena(group).master
+
+    def state_dict(self):
+        saved = super().state_dict()
+        k, steps = 0, {}
+        for gi, group in enumerate(self.param_groups):
+            arena = self._arenas.get(gi)
+            for i in range(len(group["params"])):
+                if arena is not None:
+                    steps[k] = arena.steps[i] if arena.step_dev is None else int(arena.step_dev)
+                k += 1
+        saved["state"] = {k: {"step": steps[k], **one} for k, one in saved["state"].items()}
+        return saved
+
+    def load_state_dict(self, state_dict):
+        """Takes a state_dict of an AdamW with the same groups (its state_bits and master_weights too)."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("AdamW: the saved state has other parameter groups")
+        for mine, saved in zip(self.param_groups, groups):
+            for key in ("state_bits", "master_weights"):
+                if mine[key] != saved[key]:
+                    raise ValueError(f"AdamW: the saved state has {key} {saved[key]}, this optimiser {mine[key]}")
+        plan = []
+        k = 0
+        for gi, group in enumerate(self.param_groups):
+            for i, p in enumerate(group["params"]):
+                one = state_dict["state"].get(groups[gi]["params"][i])
+                k += 1
+                if one is None:
+                    continue
+                want = [*_STATE_KEYS[group["state_bits"]]]
+                if group["master_weights"] and any(q.dtype != torch.float32 for q in group["params"]):
+                    want.append("master")
+                kind = torch.float32 if group["state_bits"] == 32 else torch.uint8
+                for key in want:
+                    shape = (_blocks(p.numel()), 2) if key == "exponents" else tuple(p.shape)
+                    dtype = {"exponents": torch.int16, "master": torch.float32}.get(key, kind)
+                    if key not in one or tuple(one[key].shape) != shape or one[key].dtype != dtype:
+                        raise ValueError(f"AdamW: the saved {key} of parameter {k - 1} is not a {dtype} of {shape}")
+                if int(one["step"]) < 0:
+                    raise ValueError(f"AdamW: the saved step of parameter {k - 1} is {one['step']}")
+                plan.append((gi, i, p, want, one))
+            if self.capturable and len({int(o["step"]) for g, _, _, _, o in plan if g == gi}) > 1:
+                raise ValueError("AdamW: with capturable=True the parameters of a group share one step")
+        self._arenas.clear()
+        self.state.clear()
+        for mine, saved in zip(self.param_groups, groups):
+            mine.update({key: val for key, val in saved.items() if key != "params"})
+            self._check_group(mine)
+        for gi, i, p, want, one in plan:
+            arena = self._arena(gi)
+            for key in want:
+                self.state[p][key].copy_(one[key])
+            arena.steps[i] = int(one["step"])
+            if arena.step_dev is not None:
+                arena.step_dev.fill_(arena.steps[i])

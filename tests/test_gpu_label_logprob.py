@@ -1,0 +1,472 @@
+"""label_log_probs (log probability of given labels, entropy, most probable classes, and the gradient)
+against the definition in 64 bits.
+
+Tolerances.  u = 2^-24 is half a step of f32.  A term e^d (d = z - max) carries the rounding of d
+(|d| u), of its product with log2 e (as much again) and of the exponential (2 u): (2|d| + 4) u of
+itself.  A sum of positive terms in chains of at most 160 (the longest in a thread, then the tree)
+adds 160 u.  With D = sum p|d| and Q = sum p d^2 that gives for s = sum e^d a relative error
+  A = u (2 D + 164),
+for log_prob = d_y - log s: A + u (2|d_y| + 4|log s| + 2|log_prob|) and for the entropy
+log s - (sum e^d d)/s: A (1 + D) + u (2 Q + 164 D + 4|log s| + 2 H).
+The gradient -p (G + g_H (log p + H)) + (the given terms): the factor's own errors times p, and
+(2|d| + 8) u + A for p itself, 4 u for its products, (k + 1) u for the sum G, and 4 u of the sizes of the given terms, which
+may cancel, for their sums.  An output of fewer
+bits adds half its step, and where it underflows half its least positive value."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import pin_slam_amd as P
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+IGNORE = -100
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm device")
+    return "cuda"
+
+
+def reference(z, y, k, g_lp=None, g_ent=None, g_top=None, ignore=IGNORE):
+    """The definition in 64 bits (z [n, C] of any type, on the CPU), and the tolerances above."""
+    zt = z.to(torch.float64)
+    n, c = zt.shape
+    z = zt.numpy()
+    y = np.asarray(y)
+    sick = ~(z < np.inf).all(1)                      # a NaN or +inf
+    m = np.where(sick, 0.0, np.where(np.isnan(z), -np.inf, z).max(1))
+    dead = m == -np.inf
+    with np.errstate(all="ignore"):
+        d = np.where((sick | dead)[:, None], 0.0, z - np.where(dead, 0.0, m)[:, None])
+        e = np.exp(d)
+        s = e.sum(1)
+        ls = np.log(s)
+        logp = d - ls[:, None]
+        p = e / s[:, None]
+        pd = np.where(p > 0, p * np.abs(np.where(p > 0, d, 0)), 0.0)
+        D = pd.sum(1)
+        Q = np.where(p > 0, pd * np.abs(np.where(p > 0, d, 0)), 0.0).sum(1)
+        ent = -np.where(p > 0, p * np.where(p > 0, logp, 0), 0.0).sum(1)
+    logp[dead] = -np.inf
+    p[dead] = 0.0
+    ent[dead] = 0.0
+    logp[sick], p[sick], ent[sick] = np.nan, np.nan, np.nan
+    has = y != ignore
+    inside = (y >= 0) & (y < c)
+    at = np.where(inside, y, 0)
+    lp = np.where(has, np.where(inside, logp[np.arange(n), at], np.nan), 0.0)
+    # value descending, class ascending; both zeros are the same value
+    order = np.argsort(-np.where(sick[:, None], 0.0, z), axis=1, kind="stable")[:, :k]
+    tlp = np.take_along_axis(logp, order, 1)
+    idx = np.where(sick[:, None], -1, order)
+    A = U * (2 * D + 164)
+    fin = lambda a: np.where(np.isfinite(a), np.abs(a), 0.0)   # noqa: E731
+    dy = fin(d[np.arange(n), at])
+    tol = {"lp": A + U * (2 * dy + 4 * fin(ls) + 2 * fin(lp)),
+           "ent": A * (1 + D) + U * (2 * Q + 164 * D + 4 * fin(ls) + 2 * fin(ent)),
+           "top": A[:, None] + U * (2 * fin(np.take_along_axis(d, order, 1)) + 4 * fin(ls)[:, None] + 2 * fin(tlp))}
+    out = {"lp": lp, "ent": ent, "top": tlp, "idx": idx}
+    if g_lp is not None or g_ent is not None or g_top is not None:
+        zero = np.zeros(n)
+        gl = np.where(has, np.where(inside, g_lp, np.nan), 0.0) if g_lp is not None else zero
+        ge = g_ent if g_ent is not None else zero
+        gt = g_top if g_top is not None else np.zeros((n, k))
+        G = gl + gt.sum(1)
+        hit = np.zeros((n, c))
+        hit[np.arange(n), at] += np.where(has, gl, 0.0)
+        np.add.at(hit, (np.arange(n)[:, None], order), gt)
+        given = np.zeros((n, c))
+        given[np.arange(n), at] += np.where(has, np.abs(gl), 0.0)
+        np.add.at(given, (np.arange(n)[:, None], order), np.abs(gt))
+        with np.errstate(all="ignore"):
+            spread = np.where(p > 0, np.where(p > 0, logp, 0) + ent[:, None], 0.0)
+            dz = -p * (G[:, None] + ge[:, None] * spread) + hit
+            size = p * (np.abs(gl) + np.abs(gt).sum(1) + 0.0)[:, None] + p * np.abs(ge)[:, None] * np.where(
+                p > 0, np.abs(np.where(p > 0, logp, 0)) + ent[:, None], 0.0)
+            rel = U * (2 * fin(d) + 12 + k) + A[:, None]
+            t = size * rel + p * np.abs(ge)[:, None] * ((tol["ent"] + A + 4 * U * fin(ls))[:, None] + 2 * U * fin(d)) \
+                + 4 * U * (given + np.abs(dz)) + 1e-37
+        dz[dead] = 0.0
+        dz[sick] = np.nan
+        t[dead] = 0.0
+        out["dz"], tol["dz"] = dz, t
+    return out, tol
+
+
+def near(got, want, tol, what):
+    got, tol = got.detach().double().cpu().numpy(), np.broadcast_to(tol, want.shape)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=what)
+    inf = np.isinf(want)
+    np.testing.assert_array_equal(got[inf], want[inf], err_msg=what)
+    ok = np.isfinite(want)
+    over = np.abs(got[ok] - want[ok]) - tol[ok]
+    assert over.size == 0 or over.max() <= 0, (what, float(over.max()), int((over > 0).sum()))
+
+
+def grad_tol(tol, dz, kind):
+    """The f32 value's tolerance and its rounding to the logits' type."""
+    if kind == torch.float32:
+        return tol
+    least = {torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[kind]
+    half = torch.finfo(kind).eps / 2
+    return tol * (1 + half) + half * np.abs(np.nan_to_num(dz)) + least / 2
+
+
+def check(logits, labels, k, grads=True, seed=0):
+    """One call (and its gradient) on the device against the reference; returns the outputs."""
+    kind = logits.dtype
+    n = logits.shape[0]
+    rng = np.random.default_rng(seed)
+    up = [rng.normal(size=n).astype(np.float32), rng.normal(size=n).astype(np.float32),
+          rng.normal(size=(n, k)).astype(np.float32)]
+    want, tol = reference(logits.cpu(), labels.cpu().numpy(), k, *[u.astype(np.float64) for u in up])
+    x = logits.detach()
+    x = x.requires_grad_(True) if grads else x
+    r = P.label_log_probs(x, labels, top_k=k, ignore_index=IGNORE)
+    assert r.log_prob.dtype == r.entropy.dtype == r.top_log_prob.dtype == torch.float32
+    assert r.top_index.dtype == torch.int64
+    near(r.log_prob, want["lp"], tol["lp"], "log_prob")
+    near(r.entropy, want["ent"], tol["ent"], "entropy")
+    np.testing.assert_array_equal(r.top_index.cpu().numpy(), want["idx"], err_msg="top_index")
+    near(r.top_log_prob, want["top"], tol["top"], "top_log_prob")
+    if grads:
+        outs = [r.log_prob, r.entropy] + ([r.top_log_prob] if k else [])
+        dz, = torch.autograd.grad(outs, x, [torch.from_numpy(u).to(x.device) for u in up[:len(outs)]])
+        assert dz.dtype == kind and dz.shape == x.shape
+        near(dz, want["dz"], grad_tol(tol["dz"], want["dz"], kind), "gradient")
+    return r
+
+
+def make(n, c, kind, dev, pad=0, seed=0, ignore_some=True):
+    g = torch.Generator().manual_seed(1000 * n + c + seed)
+    wide = torch.full((n, c + pad), math.nan)         # what lies between the rows takes no part
+    z = torch.randn((n, c), generator=g) * (0.2 + 4 * torch.rand((n, 1), generator=g)) + 5 * torch.randn((n, 1), generator=g)
+    wide[:, :c] = z
+    y = torch.randint(0, c, (n,), generator=g)
+    if ignore_some and n > 2:
+        y[::3] = IGNORE
+    return wide.to(kind).to(dev)[:, :c], y.to(dev)
+
+
+SIZES = [(1, 1), (1, 2), (2, 3), (300, 20), (1025, 19), (9, 31), (70, 32), (5, 33), (7, 63), (130, 64), (4, 65), (3, 127),
+         (11, 255), (6, 257), (513, 500), (3, 1003), (2, 2047), (5, 4097), (3, 8191), (2, 8192), (3, 16385), (2, 32769),
+         (1, 50021), (3, 65537), (1, 131072), (2, 140001)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,c", SIZES)
+def test_sizes(dev, n, c, kind):
+    for k in sorted({0, 1, min(c, 5), min(c, 32)}):
+        logits, y = make(n, c, TYPES[kind], dev, pad=(n + c) % 3, seed=k)
+        check(logits, y, k)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("pad,first", [(1, 0), (7, 3), (64, 1)])
+@pytest.mark.parametrize("c", [20, 1001, 20003])
+def test_strides_and_alignments(dev, kind, pad, first, c):
+    """Rows that begin at any element, with what is not theirs between them."""
+    n = 6
+    logits, y = make(n, c, TYPES[kind], dev)
+    wide = torch.full((n, first + c + pad), math.inf, dtype=TYPES[kind], device=dev)
+    wide[:, first:first + c] = logits
+    a = check(wide[:, first:first + c], y, 4)
+    b = P.label_log_probs(logits.contiguous(), y, top_k=4)
+    for p, q in zip(a, b):   # where a row lies does not change its values
+        torch.testing.assert_close(p.detach(), q, rtol=1e-5, atol=1e-5)
+    # classes that are not adjacent, rows that are the same, more dimensions
+    t = P.label_log_probs(logits.t().contiguous().t(), y, top_k=4)
+    assert all(torch.equal(p, q) for p, q in zip(t, b))
+    row = logits[1].expand(n, c)
+    r = P.label_log_probs(row, y, top_k=4)
+    assert torch.equal(r.entropy, r.entropy[:1].expand(n)) and torch.equal(r.top_index, r.top_index[:1].expand(n, 4))
+    v = P.label_log_probs(logits.reshape(2, 3, c), y.reshape(2, 3), top_k=4)
+    assert v.log_prob.shape == (2, 3) and v.top_index.shape == (2, 3, 4)
+    assert all(torch.equal(p.reshape(q.shape), q) for p, q in zip(v, P.label_log_probs(logits.reshape(6, c), y, top_k=4)))
+    o = P.label_log_probs(logits[2], y[2], top_k=2)
+    assert o.log_prob.shape == () and o.top_index.shape == (2,)
+
+
+def special_rows(c, kind, seed=0):
+    """Rows whose mask or values are where a softmax goes wrong, with labels for them."""
+    g = torch.Generator().manual_seed(seed + c)
+    base = torch.randn((c,), generator=g)
+    low = torch.finfo(kind).min
+    rows, labels = [], []
+
+    def add(r, y):
+        rows.append(r.clone())
+        labels.append(y)
+
+    add(torch.full((c,), -math.inf), 0)                       # nothing left
+    add(torch.full((c,), -math.inf), IGNORE)
+    add(torch.full((c,), low), c - 1)                         # masked by the type's lowest value only
+    add(torch.full((c,), torch.finfo(kind).max), 0)           # the type's largest
+    one = torch.full((c,), -math.inf)
+    one[c // 2] = 1.5
+    add(one, c // 2)                                          # one class left, and it is the label
+    add(one, 0)                                               # ... or it is not
+    few = torch.full((c,), -math.inf)
+    few[::max(1, c // 3)] = base[::max(1, c // 3)]
+    add(few, 0)                                               # fewer classes left than alternatives
+    lows = torch.full((c,), low)
+    lows[::max(1, c // 3)] = base[::max(1, c // 3)]
+    add(lows, 0)
+    add(torch.zeros(c), c // 3)                               # all equal
+    two = torch.where(base > 0, 1.0, -1.0)
+    add(two, 0)                                               # two values: many ties
+    add(torch.where(base > 0, 0.0, -0.0), 0)                  # both zeros are the same
+    add(torch.linspace(6.0, -6.0, c), 0)                      # sorted
+    add(torch.linspace(-6.0, 6.0, c), 0)
+    add(torch.linspace(-6.0, 6.0, c) * 1e-3, c - 1)
+    sharp = base.clone()
+    sharp[c - 1] = 60.0
+    add(sharp, c - 1)                                         # a sure label
+    add(sharp, 0)                                             # a hopeless one
+    add(base * 2.0 ** 10, 0)                                  # far apart
+    nan = base.clone()
+    nan[c // 2] = math.nan
+    add(nan, 0)
+    neg = torch.full((c,), -math.inf)
+    neg[0] = math.nan
+    add(neg, 0)
+    inf = base.clone()
+    inf[0] = math.inf
+    add(inf, 0)
+    add(base, -1)                                             # labels that are no class
+    add(base, c)
+    add(base, 2 ** 40)
+    add(base, IGNORE)
+    return torch.stack(rows).to(kind), torch.tensor(labels)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("c", [1, 2, 20, 64, 100, 700, 2500, 9001, 40000, 131073])
+def test_masks_ties_and_values(dev, c, kind):
+    z, y = special_rows(c, TYPES[kind])
+    for k in sorted({0, min(c, 3), min(c, 32)}):
+        check(z.to(dev), y.to(dev), k)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_large_values_in_one_place(dev, kind):
+    """All of the largest values next to one another (one lane's, one wave's, one workgroup's): the alternatives
+    come from one place, in order."""
+    c = 70001
+    z = torch.randn((8, c), generator=torch.Generator().manual_seed(7))
+    for r, a in enumerate([0, 8, 64, 500, 4096, 16000, 32768, c - 3000]):
+        z[r, a:a + 3000] = torch.linspace(50.0, 20.0, 3000) if r % 2 else torch.linspace(20.0, 50.0, 3000)
+    check(z.to(TYPES[kind]).to(dev), torch.arange(8, device=dev) * 5000, 32)
+
+
+def test_partial_gradients(dev):
+    """Each output alone, and expanded upstream gradients."""
+    logits, y = make(37, 257, torch.float32, dev)
+    full = []
+    for part in range(3):
+        x = logits.detach().clone().requires_grad_(True)
+        r = P.label_log_probs(x, y, top_k=3)
+        out = [r.log_prob, r.entropy, r.top_log_prob][part]
+        dz, = torch.autograd.grad(out.sum(), x)
+        up = [None, None, None]
+        up[part] = np.ones((37, 3) if part == 2 else 37)
+        want, tol = reference(logits.cpu(), y.cpu().numpy(), 3, *up)
+        near(dz, want["dz"], tol["dz"], f"part {part}")
+        full.append(dz)
+    x = logits.detach().clone().requires_grad_(True)
+    r = P.label_log_probs(x, y, top_k=3)
+    dz, = torch.autograd.grad(r.log_prob.sum() + r.entropy.sum() + r.top_log_prob.sum(), x)
+    torch.testing.assert_close(dz, sum(full), rtol=1e-4, atol=1e-5)
+
+
+def test_gradient_against_differences(dev):
+    """Central differences of the definition in 64 bits: error h^2/6 f''' + 2^-53 f / h, about 1e-9 at h = 1e-4
+    for logits of order 1, far below the f32 tolerance of 2e-6."""
+    n, c, k = 3, 23, 2
+    logits, y = make(n, c, torch.float32, dev, ignore_some=False)
+    logits = logits * 0.2
+    rng = np.random.default_rng(3)
+    up = [rng.normal(size=n), rng.normal(size=n), rng.normal(size=(n, k))]
+    x = logits.detach().requires_grad_(True)
+    r = P.label_log_probs(x, y, top_k=k)
+    dz, = torch.autograd.grad(list(r[:3]), x, [torch.tensor(u, dtype=torch.float32, device=dev) for u in up])
+    z0 = logits.double().cpu()
+    idx = r.top_index.cpu()
+
+    def value(z):
+        logp = z - torch.logsumexp(z, 1, keepdim=True)
+        ent = -(logp.exp() * logp).sum(1)
+        lp = logp.gather(1, y.cpu()[:, None])[:, 0]
+        return float((lp * torch.tensor(up[0])).sum() + (ent * torch.tensor(up[1])).sum()
+                     + (logp.gather(1, idx) * torch.tensor(up[2])).sum())
+
+    h = 1e-4
+    for i in range(n):
+        for j in range(c):
+            a, b = z0.clone(), z0.clone()
+            a[i, j] += h
+            b[i, j] -= h
+            assert abs((value(a) - value(b)) / (2 * h) - float(dz[i, j])) <= 2e-6 * (1 + abs(float(dz[i, j])))
+
+
+def test_same_bits_every_time(dev):
+    for n, c in [(2000, 20), (64, 1003), (3, 140001)]:
+        logits, y = make(n, c, torch.bfloat16, dev)
+        runs = []
+        for _ in range(3):
+            x = logits.detach().clone().requires_grad_(True)
+            r = P.label_log_probs(x, y, top_k=5)
+            dz, = torch.autograd.grad([r.log_prob, r.entropy], x, [torch.ones_like(r.log_prob)] * 2)
+            runs.append([*r, dz])
+        for other in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_rows_do_not_depend_on_their_number(dev):
+    """Few long rows are split over the chip, many are not: the values stay within the tolerances either way, the
+    classes are the same."""
+    logits, y = make(700, 9001, torch.float32, dev)
+    whole = P.label_log_probs(logits, y, top_k=6)
+    want, tol = reference(logits[:4].cpu(), y[:4].cpu().numpy(), 6)
+    for m in (1, 2, 4):
+        part = P.label_log_probs(logits[:m], y[:m], top_k=6)
+        assert torch.equal(part.top_index, whole.top_index[:m])
+        for r in (part, P.LabelLogProbs(*[t[:m] for t in whole])):
+            near(r.log_prob, want["lp"][:m], tol["lp"][:m], "log_prob")
+            near(r.entropy, want["ent"][:m], tol["ent"][:m], "entropy")
+
+
+def test_places_past_32_bits(dev):
+    """Rows more than 2^32 bytes and 2^31 elements apart."""
+    c, far = 1003, (1 << 31) + 24
+    buf = torch.empty((far + c,), dtype=torch.bfloat16, device=dev)
+    z = buf.as_strided((2, c), (far, 1))
+    logits, y = make(2, c, torch.bfloat16, dev)
+    z.copy_(logits)
+    got = P.label_log_probs(z, y, top_k=5)
+    want = P.label_log_probs(logits, y, top_k=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_gradient_past_32_bits(dev):
+    """A gradient of more than 2^31 elements: the last rows are the same as alone."""
+    n, c = 2200, 1000003
+    z = torch.zeros((1, c), dtype=torch.bfloat16, device=dev)
+    z[0, :1000] = torch.randn((1000,), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    x = z.expand(n, c).requires_grad_(True)
+    y = torch.arange(n, device=dev)
+    r = P.label_log_probs(x, y)
+    dz, = torch.autograd.grad(r.log_prob, x, torch.ones((n,), device=dev))
+    last = z.clone().requires_grad_(True)
+    one, = torch.autograd.grad(P.label_log_probs(last, y[-1:]).log_prob, last, torch.ones((1,), device=dev))
+    assert torch.equal(dz[-1], one[0])
+    assert float(r.log_prob[-1]) == pytest.approx(float(P.label_log_probs(z, y[-1:]).log_prob), rel=1e-5)
+
+
+def test_no_rows_and_other_label_types(dev):
+    x = torch.empty((0, 50), device=dev, requires_grad=True)
+    r = P.label_log_probs(x, torch.empty((0,), dtype=torch.int64, device=dev), top_k=2)
+    assert r.log_prob.shape == (0,) and r.top_index.shape == (0, 2)
+    dz, = torch.autograd.grad(r.log_prob.sum(), x)
+    assert dz.shape == (0, 50)
+    logits, y = make(9, 40, torch.float32, dev)
+    a = P.label_log_probs(logits, y, top_k=1)
+    b = P.label_log_probs(logits, y.to(torch.int32), top_k=1)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    other = torch.where(y == IGNORE, 39, y)
+    c = P.label_log_probs(logits, other, ignore_index=39)
+    assert torch.equal(c.log_prob[::3], torch.zeros_like(c.log_prob[::3]))
+
+
+def test_on_another_stream(dev):
+    s = torch.cuda.Stream()
+    logits, y = make(40, 5003, torch.bfloat16, dev)
+    want = P.label_log_probs(logits, y, top_k=5)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        x = (logits.float() * 1.0).to(torch.bfloat16)
+        got = P.label_log_probs(x, y, top_k=5)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_and_replayed(dev):
+    """Two graphs of forward and gradient, replayed in turn with new inputs between eager calls."""
+    graphs = []
+    for n, c in [(5, 40001), (64, 1003), (300, 20)]:
+        logits, y = make(n, c, torch.bfloat16, dev)
+        x = logits.detach().clone().requires_grad_(True)
+        up = torch.randn((n,), generator=torch.Generator().manual_seed(n)).to(dev)
+
+        def run(x=x, y=y, up=up):
+            r = P.label_log_probs(x, y, top_k=4)
+            return [t.detach() for t in r] + list(torch.autograd.grad([r.log_prob, r.entropy], x, [up, up]))
+
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, out, x, run))
+    for turn in range(4):
+        for g, out, x, run in graphs:
+            with torch.no_grad():
+                x.copy_(torch.roll(x, turn + 1, 1))
+            want = [t.clone() for t in run()]
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+def test_decoder_head_uses_it(dev):
+    """Decoder.sem_label_log_prob against the head's own log_softmax, argmax and gradient."""
+    cfg = P.Config(device=dev)
+    torch.manual_seed(5)
+    dec = P.Decoder(cfg, cfg.geo_mlp_hidden_dim, cfg.geo_mlp_level, 20)
+    x = torch.randn((500, 11), device=dev)
+    y = torch.randint(0, 20, (500,), device=dev)
+    r = dec.sem_label_log_prob(x, y, top_k=1)
+    logp = dec.sem_label_prob(x)
+    torch.testing.assert_close(r.log_prob, logp.gather(1, y[:, None])[:, 0], rtol=1e-5, atol=1e-5)
+    assert torch.equal(r.top_index[:, 0], dec.sem_label(x))
+    (-r.log_prob.mean()).backward()
+    mine = [p.grad.clone() for p in dec.parameters()]
+    dec.zero_grad()
+    torch.nn.functional.nll_loss(dec.sem_label_prob(x), y).backward()
+    for a, p in zip(mine, dec.parameters()):
+        torch.testing.assert_close(a, p.grad, rtol=1e-4, atol=1e-6)
+
+
+def test_refusals(dev):
+    z = torch.zeros((4, 10), device=dev)
+    y = torch.zeros((4,), dtype=torch.int64, device=dev)
+    for bad in (dict(top_k=11), dict(top_k=-1), dict(top_k=33)):
+        with pytest.raises(ValueError, match="top_k"):
+            P.label_log_probs(z, y, **bad)
+    with pytest.raises(ValueError, match="labels"):
+        P.label_log_probs(z, y[:3])
+    with pytest.raises(ValueError, match="whole numbers"):
+        P.label_log_probs(z, y.float())
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        P.label_log_probs(z.double(), y)
+    with pytest.raises(ValueError, match="labels on"):
+        P.label_log_probs(z, y.cpu())
+    with pytest.raises(ValueError, match="classes"):
+        P.label_log_probs(z[:, :0], y)
+    x = z.clone().requires_grad_(True)
+    r = P.label_log_probs(x, y)
+    g, = torch.autograd.grad(r.log_prob.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
