@@ -104,18 +104,18 @@ template <class T>
 __device__ __forceinline__ void store16(typename T::type* p, const uint4& q) {
     __builtin_memcpy(p, &q, 16);
 }
-// the elements [0, n) of sixteen bytes, n < N; the others -inf
+// the elements [from, to) of sixteen bytes, the others -inf
 template <class T>
-__device__ __forceinline__ uint4 load_some(const typename T::type* p, int n) {
+__device__ __forceinline__ uint4 load_some(const typename T::type* p, int from, int to) {
     uint32_t u[4] = {T::kFill, T::kFill, T::kFill, T::kFill};
     if (sizeof(typename T::type) == 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < n) __builtin_memcpy(&u[i], (const char*)p + 4 * i, 4);
+            if (i >= from && i < to) __builtin_memcpy(&u[i], (const char*)p + 4 * i, 4);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) {
+            if (i >= from && i < to) {
                 uint16_t h;
                 __builtin_memcpy(&h, (const char*)p + 2 * i, 2);
                 u[i / 2] = i & 1 ? (u[i / 2] & 0xFFFFu) | (uint32_t)h << 16 : (u[i / 2] & 0xFFFF0000u) | h;
@@ -124,14 +124,39 @@ __device__ __forceinline__ uint4 load_some(const typename T::type* p, int n) {
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// A row as aligned vectors of 16 bytes: vector u holds the classes u V - skip and on.  Its first and
+// last vector may be partly other rows'.  (Rows of an odd number of 16-bit classes, read at their own
+// alignment: 66 us for 2048 x 50021 bf16; in aligned vectors 48.)
+template <class T>
+struct Vectors {
+    const typename T::type* base;
+    int skip, classes;
+    int lo, hi;    // first and last vector that are the row's throughout (rows of 2 V classes or more have one)
+    int count;
+    __device__ __forceinline__ Vectors(const typename T::type* z, int c) : classes(c) {
+        skip = (int)((uintptr_t)z & 15) / (int)sizeof(typename T::type);
+        base = z - skip;
+        lo = skip ? 1 : 0;
+        hi = (c + skip) / T::N - 1;
+        count = (c + skip + T::N - 1) / T::N;
+    }
+    // any vector, 0 <= u: where it is not the row's throughout, another one of the row (load() puts it right)
+    __device__ __forceinline__ uint4 load_near(int u) const {
+        u = u < lo ? lo : u > hi ? hi : u;
+        return *(const uint4*)(base + (int64_t)u * T::N);
+    }
+    __device__ __forceinline__ uint4 load_edge(int u) const {
+        if (u >= count) return make_uint4(T::kFill, T::kFill, T::kFill, T::kFill);
+        const int to = classes + skip - u * T::N;
+        return load_some<T>(base + (int64_t)u * T::N, u == 0 ? skip : 0, to < T::N ? to : T::N);
+    }
+    __device__ __forceinline__ bool whole(int u) const { return u >= lo && u <= hi; }
+    __device__ __forceinline__ int first_class(int u) const { return u * T::N - skip; }
+};
+
 // The registers as they are, but unknown to the compiler: what was made of them before is made
 // again (two instructions an element) rather than kept beside them (a register an element).
 __device__ __forceinline__ void forget(uint4& q) { asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w)); }
-
-__device__ __forceinline__ int forget(int j) {
-    asm volatile("" : "+v"(j));
-    return j;
-}
 
 // ---- order: f32 values as unsigned keys in the same order, both zeros the same
 
@@ -227,98 +252,54 @@ __device__ __forceinline__ void put_top(const Out& o, const Row& r, int64_t at, 
     o.top_idx[at] = r.bad() ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
 }
 
-// One part of a row, THREADS * NCH vectors of 16 bytes held in registers.
-//
-//   1. load; maxima of vectors, threads and of 64 groups of threads
-//   2. the maximum; sum of 2^x and of 2^x x
-//   3. the k-th largest of the 64 maxima is not above the k-th largest element: what is above or
-//      at it, a little more than k, is collected in LDS and sorted by one wave
-// At most kGt larger and kEq equal elements fit.  More equal ones (rows mostly masked, or all
-// equal): the first k are found in order.  More larger ones (large values gathered in the
-// classes of few threads): k times the largest below the last.
-template <class T, int THREADS, int NCH, bool TOP>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4)
-k_label_logprob(const typename T::type* __restrict__ logits, int64_t n, int64_t classes, int64_t row_stride,
-                const int64_t* __restrict__ labels, int64_t ignore, int k, int splits, int64_t part, Out out,
-                float4* __restrict__ sums, uint64_t* __restrict__ keys) {
-    constexpr int V = T::N, W = THREADS / 64;
-    constexpr int kGt = TOP ? 4 * THREADS : 1, kEq = TOP ? 256 : 1;
-    __shared__ float s_max[64];
-    __shared__ float2 s_sum[W];
-    __shared__ uint32_t s_kth, s_gt, s_eq, s_tot[W];
-    __shared__ uint64_t s_gtk[kGt], s_eqk[kEq];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x / (unsigned)splits;
-    const int split = (int)(blockIdx.x - (unsigned)row * (unsigned)splits);
-    const int64_t first = split * part;
-    const int count = (int)(classes - first < part ? classes - first : part);   // elements of this part (may be <= 0)
-    const typename T::type* z = logits + row * row_stride + first;
-
-    uint4 q[NCH];
+// The vectors [u0, u0 + 64 W NCH) of a row up to u1, W waves, thread t's c-th being u0 + c 64 W + t, in registers.
+// All are on their way before the first is looked at.
+template <class T, int W, int NCH>
+__device__ __forceinline__ void load_part(const Vectors<T>& z, int u0, int u1, uint4 (&q)[NCH]) {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) q[c] = z.load_near(u0 + c * 64 * W + t);
+    const int last = z.hi + 1 < u1 ? z.hi + 1 : u1;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int j = (c * THREADS + tid) * V;
-        if (j + V <= count) q[c] = load16<T>(z + j);
-        else if (j < count) q[c] = load_some<T>(z + j, count - j);
-        else q[c] = make_uint4(T::kFill, T::kFill, T::kFill, T::kFill);
-    }
-    int64_t y = 0;
-    float zy = 0.f;
-    if (splits == 1 && tid == 0) {
-        y = labels[row];
-        if (y >= 0 && y < classes) zy = T::one(z + y);
-    }
-    float cm[NCH], mx = -kInf;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        float v[V];
-        T::unpack(q[c], v);
-        cm[c] = v[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) cm[c] = max_nan(cm[c], v[i]);
-        mx = max_nan(mx, cm[c]);
-    }
-    mx = mx != mx ? kInf : mx;
-    // maxima of 64 groups: threads, or the lanes of 4, or of 16
-    float g = mx;
-    if (THREADS >= 256) {
-        g = fmaxf(g, __uint_as_float(dpp<0xB1>(__float_as_uint(g))));
-        g = fmaxf(g, __uint_as_float(dpp<0x4E>(__float_as_uint(g))));
-    }
-    if (THREADS >= 1024) {
-        g = fmaxf(g, __uint_as_float(dpp<0x141>(__float_as_uint(g))));
-        g = fmaxf(g, __uint_as_float(dpp<0x140>(__float_as_uint(g))));
-    }
-    if (THREADS > 64) {
-        if (tid % (THREADS / 64) == 0) s_max[tid / (THREADS / 64)] = g;
-        if (TOP && tid == 0) s_gt = 0, s_eq = 0;
-        __syncthreads();
-        g = s_max[lane];
-    } else if (TOP && tid == 0) {
-        s_gt = 0, s_eq = 0;
-    }
-    Row r(wave_max(g));
-    if (TOP && wave == 0) {
-        // the k-th largest of the groups' maxima, bit by bit
-        const uint32_t key = order_key(g);
-        uint32_t kth = 0;
-#pragma unroll 1
-        for (int b = 31; b >= 0; --b) {
-            const uint32_t c = kth | 1u << b;
-            if (__popcll(__ballot(key >= c)) >= k) kth = c;
+        const int u = u0 + c * 64 * W + t;
+        if (u0 + (c + 1) * 64 * W > last || (c == 0 && u0 < z.lo)) {   // the same for all threads
+            if (u >= u1) q[c] = make_uint4(T::kFill, T::kFill, T::kFill, T::kFill);
+            else if (!z.whole(u)) q[c] = z.load_edge(u);
         }
-        if (lane == 0) s_kth = kth;
     }
+}
+
+// maximum of 16 bytes of logits; NaN if one is
+template <class T>
+__device__ __forceinline__ float vector_max(const uint4& q) {
+    if constexpr (__is_same(T, F16)) {   // two at a time
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        const auto two = [](uint32_t u) { return __builtin_bit_cast(v2, u); };
+        const v2 h = __builtin_elementwise_maximum(__builtin_elementwise_maximum(two(q.x), two(q.y)),
+                                                   __builtin_elementwise_maximum(two(q.z), two(q.w)));
+        return max_nan((float)h.x, (float)h.y);
+    }
+    float v[T::N];
+    T::unpack(q, v);
+    float m = v[0];
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) forget(q[c]);
-    float s = 0.f, t = 0.f;
+    for (int i = 1; i < T::N; ++i) m = max_nan(m, v[i]);
+    return m;
+}
+
+// sums of 2^x and 2^x x
+template <class T, int W, int NCH>
+__device__ __forceinline__ void part_sums(const Row& r, const uint4 (&q)[NCH], int vectors, float& s, float& t) {
+    s = t = 0.f;
     const auto add = [&](auto x_of) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            float v[V];
+            if (c > 0 && c * 64 * W >= vectors) break;   // the same for all threads
+            float v[T::N];
             T::unpack(q[c], v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < T::N; ++i) {
                 const float x = fmaxf(x_of(v[i]), kFloor);
                 const float e = __builtin_amdgcn_exp2f(x);
                 s += e;
@@ -328,170 +309,350 @@ k_label_logprob(const typename T::type* __restrict__ logits, int64_t n, int64_t 
     };
     if (!r.far) add([&](float z) { return fmaf(z, kL, -r.ml); });
     else add([&](float z) { return (z - r.m) * kL; });
+}
+
+// the k-th largest of the 64 lanes' keys, bit by bit
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
+    uint32_t kth = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t c = kth | 1u << b;
+        if (__popcll(__ballot(key >= c)) >= k) kth = c;
+    }
+    return kth;
+}
+
+// What is at or above a bound that is not above the k-th largest: two lists in LDS.
+template <int GT, int EQ>
+struct Candidates {
+    uint64_t gt[GT], eq[EQ];
+    uint32_t n_gt, n_eq;
+    __device__ __forceinline__ void push(float v, int j, float kth) {
+        if (v > kth) {
+            const uint32_t p = atomicAdd(&n_gt, 1u);
+            if (p < GT) gt[p] = class_key(v, (uint32_t)j);
+        } else if (v == kth) {
+            const uint32_t p = atomicAdd(&n_eq, 1u);
+            if (p < EQ) eq[p] = class_key(v, (uint32_t)j);
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void push_vector(const Vectors<T>& z, int u, const uint4& q, float kth) {
+        float v[T::N];
+        T::unpack(q, v);
+        const int j = z.first_class(u);
+#pragma unroll
+        for (int i = 0; i < T::N; ++i)
+            if (v[i] >= kth && j + i >= 0 && j + i < z.classes) push(v[i], j + i, kth);
+    }
+    // one wave: the k largest of the lists' g and e elements, in order; at least k
+    template <class F>
+    __device__ __forceinline__ void sort(int g, int e, int k, F emit) const {
+        const int lane = threadIdx.x & 63, all = g + e;
+        if (all <= 64) {
+            const uint64_t key = lane < g ? gt[lane] : lane < all ? eq[lane - g] : 0;
+            int rank = 0;
+            for (int i = 0; i < all; ++i) {
+                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+                rank += other > key ? 1 : 0;
+            }
+            if (lane < all && rank < k) emit(rank, key);
+            return;
+        }
+        uint64_t last = ~0ull;
+        for (int i = 0; i < k; ++i) {
+            uint64_t best = 0;
+            for (int p = lane; p < all; p += 64) {
+                const uint64_t key = p < g ? gt[p] : eq[p - g];
+                if (key < last && key > best) best = key;
+            }
+            last = wave_max_key(best);
+            if (lane == 0) emit(i, last);
+        }
+    }
+};
+
+// The first `need` classes of [from, to) whose logit is `value`, appended to eq at `have`; all threads
+// of the workgroup (THREADS of them), which may not read eq before.  Returns how many there are now.
+template <class T, int THREADS>
+__device__ __forceinline__ int first_equal(const typename T::type* z, int from, int to, float value, int need, int have,
+                                           uint64_t* eq, uint32_t* s_tot) {
+    const int wave = threadIdx.x >> 6;
+#pragma unroll 1
+    for (int j0 = from; j0 < to && have < need; j0 += THREADS) {
+        const int j = j0 + (int)threadIdx.x;
+        const float v = j < to ? T::one(z + j) : NAN;
+        const uint64_t b = __ballot(v == value);
+        int at = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if ((threadIdx.x & 63) == 0) s_tot[wave] = __popcll(b);
+        __syncthreads();
+        for (int w = 0; w < THREADS / 64; ++w) {
+            at += w < wave ? (int)s_tot[w] : 0;
+            have += (int)s_tot[w];
+        }
+        if (v == value && at < need) eq[at] = class_key(v, (uint32_t)j);
+        __syncthreads();
+    }
+    return have < need ? have : need;
+}
+
+// The k largest by k passes over the row, each the largest below the last: rows whose large logits
+// are so gathered that the lists overflow.
+template <class T, int THREADS, class F>
+__device__ __forceinline__ void largest_by_passes(const typename T::type* z, int classes, int k, uint64_t* s_key, F emit) {
+    const int wave = threadIdx.x >> 6;
+    uint64_t last = ~0ull;
+    for (int i = 0; i < k; ++i) {
+        uint64_t best = 0;
+#pragma unroll 1
+        for (int j = threadIdx.x; j < classes; j += THREADS) {
+            const uint64_t key = class_key(T::one(z + j), (uint32_t)j);
+            if (key < last && key > best) best = key;
+        }
+        best = wave_max_key(best);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s_key[wave] = best;
+        __syncthreads();
+        for (int w = 0; w < THREADS / 64; ++w) best = s_key[w] > best ? s_key[w] : best;
+        last = best;
+        if (threadIdx.x == 0) emit(i, best);
+    }
+}
+
+// One wave per row, 64 NCH vectors: the lanes' maxima, of which the k-th largest is not above the
+// row's k-th largest logit; the sums; what is at or above that, a little more than k, sorted.
+template <class T, int NCH, bool TOP>
+__global__ void __launch_bounds__(64)
+k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes, int64_t row_stride,
+             const int64_t* __restrict__ labels, int64_t ignore, int k, Out out) {
+    __shared__ Candidates<TOP ? 256 : 1, TOP ? 256 : 1> s_c;
+    __shared__ uint32_t s_tot[1];
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const typename T::type* zr = logits + row * row_stride;
+    const Vectors<T> z(zr, classes);
+    uint4 q[NCH];
+    load_part<T, 1, NCH>(z, 0, z.count, q);
+    const int64_t y = labels[row];
+    const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
+    float cm[NCH], mx = -kInf;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        cm[c] = vector_max<T>(q[c]);
+        mx = max_nan(mx, cm[c]);
+    }
+    mx = mx != mx ? kInf : mx;
+    Row r(wave_max(mx));
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) forget(q[c]);
+    float s, t;
+    part_sums<T, 1, NCH>(r, q, z.count, s, t);
     s = wave_sum(s);
     t = wave_sum(t);
-    if (THREADS > 64) {
-        if (lane == 0) s_sum[wave] = make_float2(s, t);
-        __syncthreads();
-        if (wave == 0) {
-            s = t = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) s += s_sum[w].x, t += s_sum[w].y;
-        }
-    } else if (TOP) {
-        __syncthreads();
-    }
-    r.ls = __builtin_amdgcn_logf(s);   // s >= 1 unless there is nothing
-    if (r.dead()) r.ls = 0.f;
-    const bool whole = splits == 1;
-    if (tid == 0) {
-        if (whole) {
-            out.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
-            out.entropy[row] = row_entropy(r, s, t);
-            if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
-        } else {
-            sums[blockIdx.x] = make_float4(r.m, s, t, 0.f);
-        }
+    r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);   // s >= 1 unless there is nothing
+    if (lane == 0) {
+        out.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
+        out.entropy[row] = row_entropy(r, s, t);
+        if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+        s_c.n_gt = s_c.n_eq = 0;
     }
     if (!TOP) return;
-    const int64_t at = (int64_t)blockIdx.x * k;   // of the row's outputs, or of the part's keys
-    const auto emit = [&](int i, uint64_t key) {
-        if (whole) put_top(out, r, at + i, key);
-        else keys[at + i] = key;
-    };
+    const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
     if (r.bad()) {
-        if (tid < k) emit(tid, 0);
+        if (lane < k) emit(lane, 0);
         return;
     }
-    const float kth = key_value(s_kth);
+    const float kth = key_value(kth_of_wave(order_key(mx), k));
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < NCH; ++c) forget(q[c]);
     if (mx >= kth) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            if (cm[c] >= kth) {
-                float v[V];
-                T::unpack(q[c], v);
-                const int j = forget((c * THREADS + tid) * V);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if (v[i] > kth) {
-                        const uint32_t p = atomicAdd(&s_gt, 1u);
-                        if (p < kGt) s_gtk[p] = class_key(v[i], (uint32_t)(first + j + i));
-                    } else if (v[i] == kth && j + i < count) {
-                        const uint32_t p = atomicAdd(&s_eq, 1u);
-                        if (p < kEq) s_eqk[p] = class_key(v[i], (uint32_t)(first + j + i));
-                    }
-                }
-            }
-        }
+        for (int c = 0; c < NCH; ++c)
+            if (cm[c] >= kth) s_c.push_vector(z, c * 64 + lane, q[c], kth);
     }
     __syncthreads();
-    const int gt = (int)s_gt;
-    int eq = gt >= k ? 0 : (int)s_eq;
-    // what is rare reads the part again
-    if (gt > kGt) {
-        uint64_t last = ~0ull;
-        for (int i = 0; i < k; ++i) {
-            uint64_t best = 0;
-#pragma unroll 1
-            for (int j = tid; j < count; j += THREADS) {
-                const uint64_t key = class_key(T::one(z + j), (uint32_t)(first + j));
-                if (key < last && key > best) best = key;
-            }
-            best = wave_max_key(best);
-            __syncthreads();
-            if (lane == 0) s_gtk[wave] = best;
-            __syncthreads();
-            for (int w = 0; w < W; ++w) best = s_gtk[w] > best ? s_gtk[w] : best;
-            last = best;
-            if (tid == 0) emit(i, best);
-        }
-        return;
-    }
-    if (eq > kEq) {
-        const int need = k - gt;
-        int have = 0;
-        __syncthreads();
-#pragma unroll 1
-        for (int j0 = 0; j0 < count && have < need; j0 += THREADS) {
-            const int j = j0 + tid;
-            const float v = j < count ? T::one(z + j) : NAN;
-            const uint64_t b = __ballot(v == kth);
-            int at = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-            if (lane == 0) s_tot[wave] = __popcll(b);
-            __syncthreads();
-            for (int w = 0; w < W; ++w) {
-                at += w < wave ? (int)s_tot[w] : 0;
-                have += (int)s_tot[w];
-            }
-            if (v == kth && at < need) s_eqk[at] = class_key(v, (uint32_t)(first + j));
-            __syncthreads();
-        }
-        eq = have < need ? have : need;
-    }
-    if (wave != 0) return;
-    const int all = gt + eq;
-    if (all <= 64) {
-        const uint64_t key = lane < gt ? s_gtk[lane] : lane < all ? s_eqk[lane - gt] : 0;
-        int rank = 0;
-        for (int i = 0; i < all; ++i) {
-            const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
-                                   (uint32_t)__builtin_amdgcn_readlane((int)key, i);
-            rank += other > key ? 1 : 0;
-        }
-        if (lane < all && rank < k) emit(rank, key);
-        if (lane >= all && lane < k) emit(lane, 0);   // a part of fewer than k classes
-        return;
-    }
-    uint64_t last = ~0ull;
-    for (int i = 0; i < k; ++i) {
-        uint64_t best = 0;
-        for (int p = lane; p < all; p += 64) {
-            const uint64_t key = p < gt ? s_gtk[p] : s_eqk[p - gt];
-            if (key < last && key > best) best = key;
-        }
-        last = wave_max_key(best);
-        if (lane == 0) emit(i, last);
-    }
+    const int gt = (int)s_c.n_gt;
+    int eq = gt >= k ? 0 : (int)s_c.n_eq;
+    if (gt > 256) return largest_by_passes<T, 64>(zr, classes, k, s_c.gt, emit);
+    if (eq > 256) eq = first_equal<T, 64>(zr, 0, classes, kth, k - gt, 0, s_c.eq, s_tot);
+    s_c.sort(gt, eq, k, emit);
 }
 
-// The parts of a row joined, one wave per row, one lane per part: the sums are taken to the row's
-// maximum, and the parts' sorted keys are merged.
+// A part of a long row: its maximum and sums, and for the alternatives the maxima of 64 groups of its
+// vectors (four neighbouring threads' each).
 template <class T>
-__global__ void __launch_bounds__(64)
-k_label_join(const typename T::type* __restrict__ logits, int64_t classes, int64_t row_stride,
-             const int64_t* __restrict__ labels, int64_t ignore, int k, int splits, Out out,
-             const float4* __restrict__ sums, const uint64_t* __restrict__ keys) {
-    extern __shared__ uint64_t s_keys[];
-    const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    for (int i = lane; i < splits * k; i += 64) s_keys[i] = keys[row * splits * k + i];
+__global__ void __launch_bounds__(256, 8)
+k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
+             const int64_t* __restrict__ labels, int64_t ignore, int splits, int part, Out out, float4* __restrict__ sums,
+             float* __restrict__ maxima) {
+    constexpr int NCH = 8;
+    __shared__ float s_max[4];
+    __shared__ float2 s_sum[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const unsigned row = blockIdx.x / (unsigned)splits;
+    const int u0 = (int)(blockIdx.x - row * (unsigned)splits) * part;
+    const typename T::type* zr = logits + row * row_stride;
+    const Vectors<T> z(zr, classes);
+    const int u1 = u0 + part < z.count ? u0 + part : z.count;
+    uint4 q[NCH];
+    load_part<T, 4, NCH>(z, u0, u1, q);
+    float mx = -kInf;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        if (c > 0 && u0 + c * 256 >= u1) break;
+        mx = max_nan(mx, vector_max<T>(q[c]));
+    }
+    mx = mx != mx ? kInf : mx;
+    if (maxima) {
+        float g = fmaxf(mx, __uint_as_float(dpp<0xB1>(__float_as_uint(mx))));
+        g = fmaxf(g, __uint_as_float(dpp<0x4E>(__float_as_uint(g))));
+        if ((tid & 3) == 0) maxima[(int64_t)blockIdx.x * 64 + (tid >> 2)] = g;
+    }
+    mx = wave_max(mx);
+    if (lane == 0) s_max[wave] = mx;
+    __syncthreads();
+    Row r(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) forget(q[c]);
+    float s, t;
+    part_sums<T, 4, NCH>(r, q, u1 - u0, s, t);
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (lane == 0) s_sum[wave] = make_float2(s, t);
+    __syncthreads();
+    if (tid != 0) return;
+    s = (s_sum[0].x + s_sum[1].x) + (s_sum[2].x + s_sum[3].x);
+    t = (s_sum[0].y + s_sum[1].y) + (s_sum[2].y + s_sum[3].y);
+    if (sums) {
+        sums[blockIdx.x] = make_float4(r.m, s, t, 0.f);
+        return;
+    }
+    r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
     const int64_t y = labels[row];
-    const float zy = y >= 0 && y < classes ? T::one(logits + row * row_stride + y) : 0.f;
+    out.log_prob[row] = label_log_prob(r, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
+    out.entropy[row] = row_entropy(r, s, t);
+    if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+}
+
+// The parts' sums taken to the row's maximum (one lane per part, every wave alike).
+template <class T>
+__device__ __forceinline__ Row join_sums(const float4* __restrict__ sums, const typename T::type* zr, int64_t row, int classes,
+                                         const int64_t* labels, int64_t ignore, int splits, const Out& out) {
+    const int lane = threadIdx.x & 63;
     const float4 p = lane < splits ? sums[row * splits + lane] : make_float4(-kInf, 0.f, 0.f, 0.f);
+    const int64_t y = labels[row];
+    const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
     Row r(wave_max(p.x));
     const float x = fmaxf(r.far ? (p.x - r.m) * kL : p.x * kL - r.ml, kFloor);
     const float f = __builtin_amdgcn_exp2f(x);
     const float s = wave_sum(f * p.y), t = wave_sum(f * fmaf(p.y, x, p.z));
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         out.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
         out.entropy[row] = row_entropy(r, s, t);
         if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
     }
-    if (k == 0) return;
+    return r;
+}
+
+template <class T>
+__global__ void __launch_bounds__(64)
+k_label_join(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
+             const int64_t* __restrict__ labels, int64_t ignore, int splits, Out out, const float4* __restrict__ sums) {
+    join_sums<T>(sums, logits + blockIdx.x * row_stride, blockIdx.x, classes, labels, ignore, splits, out);
+}
+
+// ... and the row's alternatives.  The k-th largest of 64 maxima of groups of groups bounds the k-th
+// largest logit from below, the k-th largest of the groups' maxima above that bound does so closer; only the
+// groups that reach it are read again (about k of them, 512 bytes each).
+template <class T>
+__global__ void __launch_bounds__(256)
+k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
+                 const int64_t* __restrict__ labels, int64_t ignore, int k, int splits, int part, Out out,
+                 const float4* __restrict__ sums, const float* __restrict__ maxima) {
+    constexpr int kGt = 1024, kEq = 256, kFew = 256;
+    __shared__ Candidates<kGt, kEq> s_c;
+    __shared__ float s_sup[64], s_val[kFew];
+    __shared__ uint16_t s_list[64 * kSplits];
+    __shared__ uint32_t s_n, s_kth, s_tot[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x;
+    const typename T::type* zr = logits + row * row_stride;
+    const Vectors<T> z(zr, classes);
+    const float* mine = maxima + row * splits * 64;
+    const int groups = splits * 64;
+    if (tid == 0) s_n = s_c.n_gt = s_c.n_eq = 0;
+    float g = -kInf;
+    for (int i = tid; i < groups; i += 256) g = fmaxf(g, mine[i]);
+    g = fmaxf(g, __uint_as_float(dpp<0xB1>(__float_as_uint(g))));
+    g = fmaxf(g, __uint_as_float(dpp<0x4E>(__float_as_uint(g))));
+    if ((tid & 3) == 0) s_sup[tid >> 2] = g;
+    const Row r = join_sums<T>(sums, zr, row, classes, labels, ignore, splits, out);
+    const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
+    if (r.bad()) {
+        if (tid < k) emit(tid, 0);
+        return;
+    }
     __syncthreads();
-    int next = 0;
-    uint64_t head = lane < splits ? s_keys[lane * k] : 0;
-    for (int i = 0; i < k; ++i) {
-        const uint64_t best = wave_max_key(head);
-        if (lane == 0) put_top(out, r, row * k + i, best);
-        if (head == best && lane < splits) {
-            ++next;
-            head = next < k ? s_keys[lane * k + next] : 0;
+    if (wave == 0) {
+        const uint32_t kth = kth_of_wave(order_key(s_sup[lane]), k);
+        if (lane == 0) s_kth = kth;
+    }
+    __syncthreads();
+    float kth = key_value(s_kth);
+    for (int i = tid; i < groups; i += 256) {
+        const float v = mine[i];
+        if (v >= kth) {
+            const uint32_t p = atomicAdd(&s_n, 1u);
+            s_list[p] = (uint16_t)i;
+            if (p < kFew) s_val[p] = v;
         }
     }
+    __syncthreads();
+    const int listed = (int)s_n;
+    if (listed > 2 * k && listed <= kFew) {   // a closer bound
+        if (wave == 0) {
+            uint32_t key[kFew / 64], c = 0;
+#pragma unroll
+            for (int i = 0; i < kFew / 64; ++i) key[i] = i * 64 + lane < listed ? order_key(s_val[i * 64 + lane]) : 0;
+#pragma unroll 1
+            for (int b = 31; b >= 0; --b) {
+                int have = 0;
+#pragma unroll
+                for (int i = 0; i < kFew / 64; ++i) have += __popcll(__ballot(key[i] >= (c | 1u << b)));
+                if (have >= k) c |= 1u << b;
+            }
+            if (lane == 0) s_kth = c;
+        }
+        __syncthreads();
+        kth = key_value(s_kth);
+    }
+    // two groups at a time per wave, one vector per lane.  With very many groups at the bound (rows mostly
+    // masked, or all equal) those that are only at it are left to first_equal.
+    const bool flood = listed > kFew;
+    const int per = (part + 255) / 256;
+    for (int i = wave * 2 + (lane >> 5); i < listed; i += 8) {
+        const int id = s_list[i], v = lane & 31;
+        const float top = mine[id];
+        const int at = (v >> 2) * 256 + (id & 63) * 4 + (v & 3), u = (id >> 6) * part + at;
+        if ((flood ? top > kth : top >= kth) && (v >> 2) < per && at < part && u < z.count)
+            s_c.push_vector(z, u, z.whole(u) ? *(const uint4*)(z.base + (int64_t)u * T::N) : z.load_edge(u), kth);
+    }
+    __syncthreads();
+    const int gt = (int)s_c.n_gt;
+    int eq = gt >= k ? 0 : (int)s_c.n_eq;
+    if (gt > kGt) return largest_by_passes<T, 256>(zr, classes, k, s_c.gt, emit);
+    if (gt < k && (flood || eq > kEq)) {
+        eq = 0;
+        for (int p = 0; p < splits && eq < k - gt; ++p) {
+            if (!(sums[row * splits + p].x >= kth)) continue;
+            const int from = z.first_class(p * part), to = z.first_class((p + 1) * part);
+            eq = first_equal<T, 256>(zr, from < 0 ? 0 : from, to < classes ? to : classes, kth, k - gt, eq, s_c.eq, s_tot);
+        }
+    }
+    if (wave == 0) s_c.sort(gt, eq, k, emit);
 }
 
 // Few classes: one thread per row, the workgroup's rows staged through LDS as f32 (an odd pitch:
@@ -669,41 +830,29 @@ bool bad_args(const void* logits, int32_t dtype, int64_t n, int64_t classes, int
     return n > 0 && (!logits || !labels || ((uintptr_t)logits & (dtype == PIN_TYPE_F32 ? 3 : 1)));
 }
 
-// How a forward is laid out: threads and vectors per thread of a workgroup, parts per row.
+// How a forward of more than kSmall classes is laid out.
 struct Plan {
-    int threads, nch, splits;
-    int64_t part;
+    int nch;       // one wave per row, nch vectors per lane; 0: parts of `part` vectors, `splits` of them
+    int splits, part;
 };
 
-constexpr int64_t kFull = 512;   // workgroups that fill the chip
+constexpr int kPart = 256 * 8;     // most vectors of a part
+constexpr int64_t kFull = 1024;    // workgroups that fill the chip
 
 Plan plan_rows(int64_t n, int64_t classes, int v) {
-    Plan p{64, 1, 1, classes};
-    const int64_t vecs = (classes + v - 1) / v;
+    const int64_t vecs = (classes + 2 * v - 2) / v;   // at any alignment
+    Plan p{1, 1, (int)vecs};
     if (vecs <= 64 * 8) {
         while (64 * p.nch < vecs) p.nch *= 2;
         return p;
     }
-    p.threads = vecs <= 256 * 8 ? 256 : 1024;
-    p.nch = 8;
-    if (p.threads == 256 && vecs <= 256 * 4) p.nch = 4;
-    if (p.threads == 1024 && vecs <= 1024 * 4) p.nch = 4;
-    int64_t s = (vecs + (int64_t)p.threads * p.nch - 1) / ((int64_t)p.threads * p.nch);
-    if (n * s < kFull && vecs > 256 * 4) {   // few rows: smaller workgroups and more parts
-        p.threads = 256;
-        p.nch = 4;
-        s = (vecs + 256 * 4 - 1) / (256 * 4);
-        if (s > kSplits) {
-            p.nch = 8;
-            s = (vecs + 256 * 8 - 1) / (256 * 8);
-        }
-        if (s > kSplits) {
-            p.threads = 1024;
-            s = (vecs + 1024 * 8 - 1) / (1024 * 8);
-        }
-    }
-    p.splits = (int)s;
-    p.part = (vecs + s - 1) / s * v;
+    p.nch = 0;
+    // no more parts than it takes, but with few rows enough to fill the chip, of two vectors per thread or more
+    int64_t s = (vecs + kPart - 1) / kPart, more = (kFull + n - 1) / n;
+    if (more > (vecs + 511) / 512) more = (vecs + 511) / 512;
+    if (more > kSplits) more = kSplits;
+    p.splits = (int)(s > more ? s : more);
+    p.part = (int)((vecs + p.splits - 1) / p.splits);
     return p;
 }
 
@@ -720,21 +869,15 @@ struct Call {
     hipStream_t st;
 };
 
-template <class T, int THREADS, int NCH>
-void launch_rows(const Call& a, const Plan& p) {
-    float4* sums = (float4*)a.ws;
-    uint64_t* keys = (uint64_t*)(sums + (p.splits > 1 ? a.n * p.splits : 0));
-    const dim3 grid((unsigned)(a.n * p.splits)), block(THREADS);
+template <class T, int NCH>
+void launch_wave(const Call& a) {
     const typename T::type* z = (const typename T::type*)a.logits;
     if (a.k > 0)
-        hipLaunchKernelGGL((k_label_logprob<T, THREADS, NCH, true>), grid, block, 0, a.st, z, a.n, a.classes, a.row_stride,
-                           a.labels, a.ignore, a.k, p.splits, p.part, a.out, sums, keys);
+        hipLaunchKernelGGL((k_label_wave<T, NCH, true>), dim3((unsigned)a.n), dim3(64), 0, a.st, z, a.n, (int)a.classes,
+                           a.row_stride, a.labels, a.ignore, a.k, a.out);
     else
-        hipLaunchKernelGGL((k_label_logprob<T, THREADS, NCH, false>), grid, block, 0, a.st, z, a.n, a.classes,
-                           a.row_stride, a.labels, a.ignore, a.k, p.splits, p.part, a.out, sums, keys);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((k_label_join<T>), dim3((unsigned)a.n), dim3(64), (size_t)p.splits * a.k * 8, a.st, z, a.classes,
-                           a.row_stride, a.labels, a.ignore, a.k, p.splits, a.out, sums, keys);
+        hipLaunchKernelGGL((k_label_wave<T, NCH, false>), dim3((unsigned)a.n), dim3(64), 0, a.st, z, a.n, (int)a.classes,
+                           a.row_stride, a.labels, a.ignore, a.k, a.out);
 }
 
 template <class T>
@@ -755,19 +898,26 @@ int run_forward(const Call& a) {
     }
     const Plan p = plan_rows(a.n, a.classes, T::N);
     if (a.n * p.splits > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
-    if (p.splits > 1 && (!a.ws || ((uintptr_t)a.ws & 15))) return PIN_ERR_ARG;
-    if (p.threads == 64) {
-        if (p.nch == 1) launch_rows<T, 64, 1>(a, p);
-        else if (p.nch == 2) launch_rows<T, 64, 2>(a, p);
-        else if (p.nch == 4) launch_rows<T, 64, 4>(a, p);
-        else launch_rows<T, 64, 8>(a, p);
-    } else if (p.threads == 256) {
-        if (p.nch == 4) launch_rows<T, 256, 4>(a, p);
-        else launch_rows<T, 256, 8>(a, p);
-    } else {
-        if (p.nch == 4) launch_rows<T, 1024, 4>(a, p);
-        else launch_rows<T, 1024, 8>(a, p);
+    if (p.nch > 0) {
+        if (p.nch == 1) launch_wave<T, 1>(a);
+        else if (p.nch == 2) launch_wave<T, 2>(a);
+        else if (p.nch == 4) launch_wave<T, 4>(a);
+        else launch_wave<T, 8>(a);
+        return launch_status();
     }
+    const typename T::type* z = (const typename T::type*)a.logits;
+    const bool join = p.splits > 1 || a.k > 0;
+    if (join && (!a.ws || ((uintptr_t)a.ws & 15))) return PIN_ERR_ARG;
+    float4* sums = join ? (float4*)a.ws : nullptr;
+    float* maxima = a.k > 0 ? (float*)(sums + a.n * p.splits) : nullptr;
+    hipLaunchKernelGGL((k_label_part<T>), dim3((unsigned)(a.n * p.splits)), dim3(256), 0, a.st, z, (int)a.classes,
+                       a.row_stride, a.labels, a.ignore, p.splits, p.part, a.out, sums, maxima);
+    if (a.k > 0)
+        hipLaunchKernelGGL((k_label_join_top<T>), dim3((unsigned)a.n), dim3(256), 0, a.st, z, (int)a.classes, a.row_stride,
+                           a.labels, a.ignore, a.k, p.splits, p.part, a.out, sums, maxima);
+    else if (join)
+        hipLaunchKernelGGL((k_label_join<T>), dim3((unsigned)a.n), dim3(64), 0, a.st, z, (int)a.classes, a.row_stride,
+                           a.labels, a.ignore, p.splits, a.out, sums);
     return launch_status();
 }
 
@@ -822,7 +972,7 @@ int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dt
         return PIN_ERR_ARG;
     if (n == 0 || classes <= kSmall) return 0;
     const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N);
-    return p.splits > 1 ? n * p.splits * (16 + 8 * (int64_t)top_k) : 0;
+    return p.nch > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
 }
 
 int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
