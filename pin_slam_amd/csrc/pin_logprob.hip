@@ -482,12 +482,11 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
 
 // A part of a long row: its maximum and sums, and for the alternatives the maxima of 64 groups of its
 // vectors (four neighbouring threads' each).
-template <class T>
+template <class T, int NCH>
 __global__ void __launch_bounds__(256, 8)
 k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
              const int64_t* __restrict__ labels, int64_t ignore, int splits, int part, Out out, float4* __restrict__ sums,
              float* __restrict__ maxima) {
-    constexpr int NCH = 8;
     __shared__ float s_max[4];
     __shared__ float2 s_sum[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -564,59 +563,48 @@ k_label_join(const typename T::type* __restrict__ logits, int classes, int64_t r
     join_sums<T>(sums, logits + blockIdx.x * row_stride, blockIdx.x, classes, labels, ignore, splits, out);
 }
 
-// ... and the row's alternatives.  The k-th largest of 64 maxima of groups of groups bounds the k-th
-// largest logit from below, the k-th largest of the groups' maxima above that bound does so closer; only the
-// groups that reach it are read again (about k of them, 512 bytes each).
-template <class T>
-__global__ void __launch_bounds__(256)
-k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
-                 const int64_t* __restrict__ labels, int64_t ignore, int k, int splits, int part, Out out,
-                 const float4* __restrict__ sums, const float* __restrict__ maxima) {
-    constexpr int kGt = 1024, kEq = 256, kFew = 256;
-    __shared__ Candidates<kGt, kEq> s_c;
-    __shared__ float s_sup[64], s_val[kFew];
-    __shared__ uint16_t s_list[64 * kSplits];
-    __shared__ uint32_t s_n, s_kth, s_tot[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x;
-    const typename T::type* zr = logits + row * row_stride;
-    const Vectors<T> z(zr, classes);
-    const float* mine = maxima + row * splits * 64;
-    const int groups = splits * 64;
-    if (tid == 0) s_n = s_c.n_gt = s_c.n_eq = 0;
-    float g = -kInf;
-    for (int i = tid; i < groups; i += 256) g = fmaxf(g, mine[i]);
-    g = fmaxf(g, __uint_as_float(dpp<0xB1>(__float_as_uint(g))));
-    g = fmaxf(g, __uint_as_float(dpp<0x4E>(__float_as_uint(g))));
-    if ((tid & 3) == 0) s_sup[tid >> 2] = g;
-    const Row r = join_sums<T>(sums, zr, row, classes, labels, ignore, splits, out);
-    const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
-    if (r.bad()) {
-        if (tid < k) emit(tid, 0);
-        return;
-    }
-    __syncthreads();
+// The alternatives of a row from the maxima of its groups (64 per part of `part` vectors: group i of a part
+// holds the vectors 256 c + 4 i .. 4 i + 3), and the maxima of 64 groups of groups.  The k-th largest of the
+// latter bounds the k-th largest logit from below, the k-th largest of the groups' maxima above that bound
+// does so closer; only the groups that reach it are read again, about k of them.
+struct TopSpace {
+    static constexpr int kGt = 512, kEq = 128, kFew = 256;
+    Candidates<kGt, kEq> c;
+    float sup[64], val[kFew];
+    uint16_t list[kFew];
+    uint32_t n, kth, tot[4];
+    __device__ __forceinline__ void clear() { n = c.n_gt = c.n_eq = 0; }   // one thread, before a barrier
+};
+
+// 256 threads; m.sup and the maxima are written, with a barrier behind them
+template <class T, class F>
+__device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int parts, int part, const Vectors<T>& z,
+                                           const typename T::type* zr, int k, F emit) {
+    constexpr int kFew = TopSpace::kFew, W = 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = parts * 64;
     if (wave == 0) {
-        const uint32_t kth = kth_of_wave(order_key(s_sup[lane]), k);
-        if (lane == 0) s_kth = kth;
+        const uint32_t kth = kth_of_wave(order_key(m.sup[lane]), k);
+        if (lane == 0) m.kth = kth;
     }
     __syncthreads();
-    float kth = key_value(s_kth);
+    float kth = key_value(m.kth);
     for (int i = tid; i < groups; i += 256) {
-        const float v = mine[i];
+        const float v = maxima[i];
         if (v >= kth) {
-            const uint32_t p = atomicAdd(&s_n, 1u);
-            s_list[p] = (uint16_t)i;
-            if (p < kFew) s_val[p] = v;
+            const uint32_t p = atomicAdd(&m.n, 1u);
+            if (p < kFew) m.val[p] = v, m.list[p] = (uint16_t)i;
         }
     }
     __syncthreads();
-    const int listed = (int)s_n;
-    if (listed > 2 * k && listed <= kFew) {   // a closer bound
+    const int listed = (int)m.n;
+    // with very many groups at the bound (rows mostly masked, or all equal) those that are only at it are
+    // left to first_equal
+    const bool flood = listed > kFew;
+    if (listed > 2 * k && !flood) {   // a closer bound
         if (wave == 0) {
             uint32_t key[kFew / 64], c = 0;
 #pragma unroll
-            for (int i = 0; i < kFew / 64; ++i) key[i] = i * 64 + lane < listed ? order_key(s_val[i * 64 + lane]) : 0;
+            for (int i = 0; i < kFew / 64; ++i) key[i] = i * 64 + lane < listed ? order_key(m.val[i * 64 + lane]) : 0;
 #pragma unroll 1
             for (int b = 31; b >= 0; --b) {
                 int have = 0;
@@ -624,35 +612,171 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
                 for (int i = 0; i < kFew / 64; ++i) have += __popcll(__ballot(key[i] >= (c | 1u << b)));
                 if (have >= k) c |= 1u << b;
             }
-            if (lane == 0) s_kth = c;
+            if (lane == 0) m.kth = c;
         }
         __syncthreads();
-        kth = key_value(s_kth);
+        kth = key_value(m.kth);
     }
-    // two groups at a time per wave, one vector per lane.  With very many groups at the bound (rows mostly
-    // masked, or all equal) those that are only at it are left to first_equal.
-    const bool flood = listed > kFew;
-    const int per = (part + 255) / 256;
-    for (int i = wave * 2 + (lane >> 5); i < listed; i += 8) {
-        const int id = s_list[i], v = lane & 31;
-        const float top = mine[id];
-        const int at = (v >> 2) * 256 + (id & 63) * 4 + (v & 3), u = (id >> 6) * part + at;
-        if ((flood ? top > kth : top >= kth) && (v >> 2) < per && at < part && u < z.count)
-            s_c.push_vector(z, u, z.whole(u) ? *(const uint4*)(z.base + (int64_t)u * T::N) : z.load_edge(u), kth);
+    // two groups at a time per wave, one vector per lane, four reads on their way
+    constexpr int R = 4;
+    const int per = (part + 255) / 256, some = flood ? groups : listed;
+    for (int i0 = wave * 2 + (lane >> 5); i0 < some; i0 += 2 * W * R) {
+        uint4 q[R];
+        int at[R];
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+            const int i = i0 + e * 2 * W, v = lane & 31;
+            at[e] = -1;
+            if (i < some) {
+                const int id = flood ? i : m.list[i];
+                const float top = flood ? maxima[id] : m.val[i];
+                const int in = (v >> 2) * 256 + (id & 63) * 4 + (v & 3), u = (id >> 6) * part + in;
+                if ((flood ? top > kth : top >= kth) && (v >> 2) < per && in < part && u < z.count) at[e] = u;
+            }
+            q[e] = z.load_near(at[e] < 0 ? 0 : at[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < R; ++e)
+            if (at[e] >= 0) m.c.push_vector(z, at[e], z.whole(at[e]) ? q[e] : z.load_edge(at[e]), kth);
     }
     __syncthreads();
-    const int gt = (int)s_c.n_gt;
-    int eq = gt >= k ? 0 : (int)s_c.n_eq;
-    if (gt > kGt) return largest_by_passes<T, 256>(zr, classes, k, s_c.gt, emit);
-    if (gt < k && (flood || eq > kEq)) {
+    const int gt = (int)m.c.n_gt;
+    int eq = gt >= k ? 0 : (int)m.c.n_eq;
+    if (gt > TopSpace::kGt) return largest_by_passes<T, 256>(zr, z.classes, k, m.c.gt, emit);
+    if (gt < k && (flood || eq > TopSpace::kEq)) {
         eq = 0;
-        for (int p = 0; p < splits && eq < k - gt; ++p) {
-            if (!(sums[row * splits + p].x >= kth)) continue;
+        for (int p = 0; p < parts && eq < k - gt; ++p) {
+            if (!__any(maxima[p * 64 + lane] >= kth)) continue;
             const int from = z.first_class(p * part), to = z.first_class((p + 1) * part);
-            eq = first_equal<T, 256>(zr, from < 0 ? 0 : from, to < classes ? to : classes, kth, k - gt, eq, s_c.eq, s_tot);
+            eq = first_equal<T, 256>(zr, from < 0 ? 0 : from, to < z.classes ? to : z.classes, kth, k - gt, eq, m.c.eq,
+                                     m.tot);
         }
     }
-    if (wave == 0) s_c.sort(gt, eq, k, emit);
+    if (wave == 0) m.c.sort(gt, eq, k, emit);
+}
+
+// a thread's maximum to its four neighbours', and those of a workgroup's 64 fours to `to`
+__device__ __forceinline__ void put_fours(float v, float* to) {
+    v = fmaxf(v, __uint_as_float(dpp<0xB1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(dpp<0x4E>(__float_as_uint(v))));
+    if ((threadIdx.x & 3) == 0) to[threadIdx.x >> 2] = v;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
+                 const int64_t* __restrict__ labels, int64_t ignore, int k, int splits, int part, Out out,
+                 const float4* __restrict__ sums, const float* __restrict__ maxima) {
+    __shared__ TopSpace s_m;
+    const int64_t row = blockIdx.x;
+    const typename T::type* zr = logits + row * row_stride;
+    const float* mine = maxima + row * splits * 64;
+    if (threadIdx.x == 0) s_m.clear();
+    float g = -kInf;
+    for (int i = threadIdx.x; i < splits * 64; i += 256) g = fmaxf(g, mine[i]);
+    put_fours(g, s_m.sup);
+    const Row r = join_sums<T>(sums, zr, row, classes, labels, ignore, splits, out);
+    const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
+    if (r.bad()) {
+        if ((int)threadIdx.x < k) emit(threadIdx.x, 0);
+        return;
+    }
+    __syncthreads();
+    top_of_row<T>(s_m, mine, splits, part, Vectors<T>(zr, classes), zr, k, emit);
+}
+
+// Many long rows: a workgroup goes through a row alone, kPart vectors at a time, each thread with a running
+// maximum of its own (2^x is taken to it, and what it has summed is taken to a new one), so nothing waits
+// for the other threads before the row's end.
+constexpr int kPart = 256 * 4;     // vectors of a part
+constexpr int kRowParts = 32;      // most parts of a row here (their groups' maxima lie in LDS)
+
+template <class T>
+__global__ void __launch_bounds__(256, 8)
+k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
+            const int64_t* __restrict__ labels, int64_t ignore, int k, int parts, Out out) {
+    constexpr int NCH = kPart / 256;
+    __shared__ TopSpace s_m;
+    __shared__ float s_max[kRowParts * 64];
+    __shared__ float4 s_sum[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x;
+    const typename T::type* zr = logits + row * row_stride;
+    const Vectors<T> z(zr, classes);
+    if (tid == 0) s_m.clear();
+    constexpr float kLow = -0x1p126f;
+    float m = -kInf, ml = kLow * kL, s = 0.f, t = 0.f;
+#pragma unroll 1
+    for (int p = 0; p < parts; ++p) {
+        const int u0 = p * kPart, u1 = u0 + kPart < z.count ? u0 + kPart : z.count;
+        uint4 q[NCH];
+        load_part<T, 4, NCH>(z, u0, u1, q);
+        float mx = vector_max<T>(q[0]);
+#pragma unroll
+        for (int c = 1; c < NCH; ++c) mx = max_nan(mx, vector_max<T>(q[c]));
+        mx = mx != mx ? kInf : mx;
+        put_fours(mx, s_max + p * 64);
+        if (__any(mx > m)) {
+            m = fmaxf(m, mx);
+            const float to = fmaxf(m, kLow) * kL, x = fmaxf(ml - to, kFloor), f = __builtin_amdgcn_exp2f(x);
+            t = f * fmaf(s, x, t);
+            s *= f;
+            ml = to;
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) forget(q[c]);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            if (c > 0 && u0 + c * 256 >= u1) break;
+            float v[T::N];
+            T::unpack(q[c], v);
+#pragma unroll
+            for (int i = 0; i < T::N; ++i) {
+                const float x = fmaxf(fmaf(v[i], kL, -ml), kFloor);
+                const float e = __builtin_amdgcn_exp2f(x);
+                s += e;
+                t = fmaf(e, x, t);
+            }
+        }
+    }
+    put_fours(m, s_m.sup);
+    const float wm = wave_max(m);
+    if (lane == 0) s_sum[wave].z = wm;
+    __syncthreads();
+    Row r(fmaxf(fmaxf(s_sum[0].z, s_sum[1].z), fmaxf(s_sum[2].z, s_sum[3].z)));
+    if (fabsf(r.m) > 0x1p126f && !r.bad() && !r.dead()) {   // no thread's maximum was one to take 2^x to
+        s = t = 0.f;
+        r.far = true;
+        for (int j = tid; j < classes; j += 256) {
+            const float x = fmaxf(r.x(T::one(zr + j)), kFloor), e = __builtin_amdgcn_exp2f(x);
+            s += e;
+            t = fmaf(e, x, t);
+        }
+    } else {
+        const float x = fmaxf(ml - r.ml, kFloor), f = __builtin_amdgcn_exp2f(x);
+        t = f * fmaf(s, x, t);
+        s *= f;
+    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (lane == 0) s_sum[wave].x = s, s_sum[wave].y = t;
+    __syncthreads();
+    s = (s_sum[0].x + s_sum[1].x) + (s_sum[2].x + s_sum[3].x);
+    t = (s_sum[0].y + s_sum[1].y) + (s_sum[2].y + s_sum[3].y);
+    r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
+    if (tid == 0) {
+        const int64_t y = labels[row];
+        out.log_prob[row] = label_log_prob(r, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
+        out.entropy[row] = row_entropy(r, s, t);
+        if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+    }
+    if (k == 0) return;
+    const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
+    if (r.bad()) {
+        if (tid < k) emit(tid, 0);
+        return;
+    }
+    top_of_row<T>(s_m, s_max, parts, kPart, z, zr, k, emit);
 }
 
 // Few classes: one thread per row, the workgroup's rows staged through LDS as f32 (an odd pitch:
@@ -834,21 +958,30 @@ bool bad_args(const void* logits, int32_t dtype, int64_t n, int64_t classes, int
 struct Plan {
     int nch;       // one wave per row, nch vectors per lane; 0: parts of `part` vectors, `splits` of them
     int splits, part;
+    int alone;     // a workgroup goes through a row alone, this many parts
 };
 
-constexpr int kPart = 256 * 8;     // most vectors of a part
 constexpr int64_t kFull = 1024;    // workgroups that fill the chip
+constexpr int64_t kRows = 2048;    // rows that do when each has a workgroup
 
 Plan plan_rows(int64_t n, int64_t classes, int v) {
     const int64_t vecs = (classes + 2 * v - 2) / v;   // at any alignment
-    Plan p{1, 1, (int)vecs};
+    Plan p{1, 1, (int)vecs, 0};
     if (vecs <= 64 * 8) {
         while (64 * p.nch < vecs) p.nch *= 2;
         return p;
     }
     p.nch = 0;
+    const int64_t parts = (vecs + kPart - 1) / kPart;
+    if (n >= kRows && parts <= kRowParts) {
+        p.part = kPart;
+        p.alone = (int)parts;
+        return p;
+    }
     // no more parts than it takes, but with few rows enough to fill the chip, of two vectors per thread or more
-    int64_t s = (vecs + kPart - 1) / kPart, more = (kFull + n - 1) / n;
+    int64_t s = (vecs + kPart - 1) / kPart;
+    if (s > kSplits) s = (vecs + 2 * kPart - 1) / (2 * kPart);
+    int64_t more = (kFull + n - 1) / n;
     if (more > (vecs + 511) / 512) more = (vecs + 511) / 512;
     if (more > kSplits) more = kSplits;
     p.splits = (int)(s > more ? s : more);
@@ -906,15 +1039,25 @@ int run_forward(const Call& a) {
         return launch_status();
     }
     const typename T::type* z = (const typename T::type*)a.logits;
+    if (p.alone > 0) {
+        hipLaunchKernelGGL((k_label_row<T>), dim3((unsigned)a.n), dim3(256), 0, a.st, z, (int)a.classes, a.row_stride,
+                           a.labels, a.ignore, a.k, p.alone, a.out);
+        return launch_status();
+    }
     const bool join = p.splits > 1 || a.k > 0;
     if (join && (!a.ws || ((uintptr_t)a.ws & 15))) return PIN_ERR_ARG;
     float4* sums = join ? (float4*)a.ws : nullptr;
     float* maxima = a.k > 0 ? (float*)(sums + a.n * p.splits) : nullptr;
-    hipLaunchKernelGGL((k_label_part<T>), dim3((unsigned)(a.n * p.splits)), dim3(256), 0, a.st, z, (int)a.classes,
-                       a.row_stride, a.labels, a.ignore, p.splits, p.part, a.out, sums, maxima);
+    const dim3 grid((unsigned)(a.n * p.splits)), rows((unsigned)a.n);
+    if (p.part <= kPart)
+        hipLaunchKernelGGL((k_label_part<T, 4>), grid, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
+                           a.ignore, p.splits, p.part, a.out, sums, maxima);
+    else
+        hipLaunchKernelGGL((k_label_part<T, 8>), grid, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
+                           a.ignore, p.splits, p.part, a.out, sums, maxima);
     if (a.k > 0)
-        hipLaunchKernelGGL((k_label_join_top<T>), dim3((unsigned)a.n), dim3(256), 0, a.st, z, (int)a.classes, a.row_stride,
-                           a.labels, a.ignore, a.k, p.splits, p.part, a.out, sums, maxima);
+        hipLaunchKernelGGL((k_label_join_top<T>), rows, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
+                           a.ignore, a.k, p.splits, p.part, a.out, sums, maxima);
     else if (join)
         hipLaunchKernelGGL((k_label_join<T>), dim3((unsigned)a.n), dim3(64), 0, a.st, z, (int)a.classes, a.row_stride,
                            a.labels, a.ignore, p.splits, a.out, sums);
@@ -972,7 +1115,7 @@ int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dt
         return PIN_ERR_ARG;
     if (n == 0 || classes <= kSmall) return 0;
     const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N);
-    return p.nch > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
+    return p.nch > 0 || p.alone > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
 }
 
 int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
