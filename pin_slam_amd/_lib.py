@@ -231,7 +231,7 @@ _SIGS = {
                           c_void_p, c_void_p, c_void_p],
     "pin_label_logprob_bwd": [c_void_p, i32, i64, i64, i64, c_void_p, i64, i32, c_void_p, c_void_p, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_void_p],
-    "pin_adamw_step": [_P(c_void_p), _P(c_void_p), _P(i64), _P(i64), i32, i32, i32, c_void_p, c_void_p, c_void_p,
+    "pin_adamw_step": [c_void_p, c_void_p, c_void_p, c_void_p, i32, i32, i32, c_void_p, c_void_p, c_void_p,
                        c_void_p, i64, f64, f64, f64, f64, f64, i64, u32, c_void_p, c_void_p],
     "pin_adamw_scalars": [c_void_p, c_void_p, f64, f64, f64, f64, u32, c_void_p, c_void_p],
     "pin_adamw_moments": [c_void_p, c_void_p, c_void_p, i64, c_void_p, c_void_p, c_void_p],

@@ -38,6 +38,7 @@ struct F32 {
     typedef float type;
     static constexpr int N = 4;
     static constexpr uint32_t kFill = 0xFF800000u;   // -inf in every element
+    static constexpr int kLow = 0;                   // even number of low bits that are the same in all f32 values
     static __device__ __forceinline__ void unpack(const uint4& q, float (&o)[4]) {
         o[0] = __uint_as_float(q.x), o[1] = __uint_as_float(q.y), o[2] = __uint_as_float(q.z), o[3] = __uint_as_float(q.w);
     }
@@ -53,6 +54,7 @@ struct F16 {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr int N = 8;
     static constexpr uint32_t kFill = 0xFC00FC00u;
+    static constexpr int kLow = 12;
     static __device__ __forceinline__ void unpack(const uint4& q, float (&o)[8]) {
         const v8 h = __builtin_bit_cast(v8, q);
 #pragma unroll
@@ -73,6 +75,7 @@ struct BF16 {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr int N = 8;
     static constexpr uint32_t kFill = 0xFF80FF80u;
+    static constexpr int kLow = 16;
     static __device__ __forceinline__ void unpack(const uint4& q, float (&o)[8]) {
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -311,15 +314,29 @@ __device__ __forceinline__ void part_sums(const Row& r, const uint4 (&q)[NCH], i
     else add([&](float z) { return (z - r.m) * kL; });
 }
 
-// the k-th largest of the 64 lanes' keys, bit by bit
-__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
+// The k-th largest of the wave's keys, N in each lane, two bits at a time.  LOW: bits that are alike in all
+// keys of a sign (a 16-bit type's: 0 of positive values, 1 of negative ones).
+template <int LOW, int N>
+__device__ __forceinline__ uint32_t kth_of_wave(const uint32_t (&key)[N], int k) {
+    const auto count = [&](uint32_t c) {
+        int have = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) have += __popcll(__ballot(key[i] >= c));
+        return have;
+    };
     uint32_t kth = 0;
 #pragma unroll 1
-    for (int b = 31; b >= 0; --b) {
-        const uint32_t c = kth | 1u << b;
-        if (__popcll(__ballot(key >= c)) >= k) kth = c;
+    for (int b = 30; b >= LOW; b -= 2) {
+        const uint32_t one = kth | 1u << b, two = kth | 2u << b, three = kth | 3u << b;
+        const int n1 = count(one), n2 = count(two), n3 = count(three);
+        kth = n3 >= k ? three : n2 >= k ? two : n1 >= k ? one : kth;
     }
-    return kth;
+    return LOW == 0 || kth & 0x80000000u ? kth : kth | ((1u << LOW) - 1);
+}
+template <int LOW>
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
+    const uint32_t one[1] = {key};
+    return kth_of_wave<LOW, 1>(one, k);
 }
 
 // What is at or above a bound that is not above the k-th largest: two lists in LDS.
@@ -463,7 +480,7 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
         if (lane < k) emit(lane, 0);
         return;
     }
-    const float kth = key_value(kth_of_wave(order_key(mx), k));
+    const float kth = key_value(kth_of_wave<T::kLow>(order_key(mx), k));
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < NCH; ++c) forget(q[c]);
@@ -583,7 +600,7 @@ __device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int
     constexpr int kFew = TopSpace::kFew, W = 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = parts * 64;
     if (wave == 0) {
-        const uint32_t kth = kth_of_wave(order_key(m.sup[lane]), k);
+        const uint32_t kth = kth_of_wave<T::kLow>(order_key(m.sup[lane]), k);
         if (lane == 0) m.kth = kth;
     }
     __syncthreads();
@@ -602,16 +619,10 @@ __device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int
     const bool flood = listed > kFew;
     if (listed > 2 * k && !flood) {   // a closer bound
         if (wave == 0) {
-            uint32_t key[kFew / 64], c = 0;
+            uint32_t key[kFew / 64];
 #pragma unroll
             for (int i = 0; i < kFew / 64; ++i) key[i] = i * 64 + lane < listed ? order_key(m.val[i * 64 + lane]) : 0;
-#pragma unroll 1
-            for (int b = 31; b >= 0; --b) {
-                int have = 0;
-#pragma unroll
-                for (int i = 0; i < kFew / 64; ++i) have += __popcll(__ballot(key[i] >= (c | 1u << b)));
-                if (have >= k) c |= 1u << b;
-            }
+            const uint32_t c = kth_of_wave<T::kLow>(key, k);
             if (lane == 0) m.kth = c;
         }
         __syncthreads();
@@ -962,7 +973,7 @@ struct Plan {
 };
 
 constexpr int64_t kFull = 1024;    // workgroups that fill the chip
-constexpr int64_t kRows = 2048;    // rows that do when each has a workgroup
+constexpr int64_t kRows = 256;     // rows that do when each has a workgroup
 
 Plan plan_rows(int64_t n, int64_t classes, int v) {
     const int64_t vecs = (classes + 2 * v - 2) / v;   // at any alignment
@@ -973,7 +984,7 @@ Plan plan_rows(int64_t n, int64_t classes, int v) {
     }
     p.nch = 0;
     const int64_t parts = (vecs + kPart - 1) / kPart;
-    if (n >= kRows && parts <= kRowParts) {
+    if (parts <= kRowParts && (n >= kRows || parts <= 2)) {
         p.part = kPart;
         p.alone = (int)parts;
         return p;

@@ -18,17 +18,19 @@ LabelLogProbs = namedtuple("LabelLogProbs", ["log_prob", "entropy", "top_log_pro
 def _forward(z, y, k, ignore, want_stats):
     n, c = z.shape
     dev = z.device
-    lp = torch.empty((n,), dtype=torch.float32, device=dev)
-    ent = torch.empty((n,), dtype=torch.float32, device=dev)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
-    tlp = torch.empty((n, k), dtype=torch.float32, device=dev)
+    # one allocation for what is f32: the two columns, the statistics, the alternatives
+    buf = torch.empty((2 * n * (1 + want_stats) + n * k,), dtype=torch.float32, device=dev)
+    at = 2 * n * (1 + want_stats)
+    lp, ent, stats, tlp = buf[:n], buf[n:2 * n], buf[2 * n:at] if want_stats else None, buf[at:].view(n, k)
     tidx = torch.empty((n, k), dtype=torch.int64, device=dev)
     dt = _lib.TYPES[z.dtype]
+    base = buf.data_ptr()
     with _lib.on_device(dev):
         need = _lib.fn("pin_label_logprob_workspace_bytes")(n, c, dt, k)
         ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-        _lib.call("pin_label_logprob", z.data_ptr(), dt, n, c, z.stride(0), _lib.ptr(y), ignore, k, _lib.ptr(lp),
-                  _lib.ptr(ent), _lib.ptr(stats), _lib.ptr(tlp), _lib.ptr(tidx), _lib.ptr(ws), _lib.stream(dev))
+        _lib.call("pin_label_logprob", z.data_ptr(), dt, n, c, z.stride(0), y.data_ptr(), ignore, k, base, base + 4 * n,
+                  base + 8 * n if want_stats else None, base + 4 * at if k else None, tidx.data_ptr() if k else None,
+                  None if ws is None else ws.data_ptr(), _lib.stream(dev))
     return lp, ent, stats, tlp, tidx
 
 

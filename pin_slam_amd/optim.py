@@ -11,7 +11,7 @@ of 256 elements (``offsets``); ``state[p]`` holds views of them.  With state_bit
 one byte per element and two bytes per 256, rounded so that its expectation is kept
 (csrc/pin_adamw.hip).
 """
-import ctypes
+from array import array
 
 import torch
 
@@ -49,6 +49,9 @@ class _Arena:
             for p, a, n in zip(params, self.offsets, self.sizes):
                 self.master[a:a + n] = p.detach().reshape(-1)
         self.steps = [0] * len(params)
+        self.together = True              # all of them are the same
+        self.where, self.kinds = None, set()   # the parameters as they were last checked one by one
+        self.c_sizes, self.c_offsets = array("q", self.sizes), array("q", self.offsets)
         # a step that a graph may replay counts on the device, all of the group's parameters together
         self.step_dev = torch.zeros((1,), dtype=torch.int64, device=dev) if capturable else None
         self.scalars = torch.zeros((_lib.ADAMW_SCALARS_BYTES,), dtype=torch.uint8, device=dev) if capturable else None
@@ -141,23 +144,42 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: parameters were added to or taken from a group after its first step")
         return arena
 
+    def _check(self, arena, i, p, g):
+        """One parameter and its gradient; the gradient as the kernel takes it."""
+        if g.layout != torch.strided:
+            raise RuntimeError("AdamW: sparse gradients are not implemented")
+        if p.numel() != arena.sizes[i] or p.device != arena.device or not p.is_contiguous():
+            raise RuntimeError("AdamW: a parameter was reshaped or moved after its first step")
+        if g.dtype != p.dtype or g.device != arena.device or p.dtype not in _lib.TYPES or g.numel() != arena.sizes[i]:
+            raise RuntimeError(f"AdamW: a {p.dtype} parameter on {p.device} has a {g.dtype} gradient on {g.device}")
+        return g if g.is_contiguous() else g.contiguous()
+
     def _gather(self, arena, group):
-        """Indexes, parameters and gradients of what has a gradient, checked."""
-        todo = []
-        for i, p in enumerate(group["params"]):
-            g = p.grad
-            if g is None:
-                if self.capturable:
-                    raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
-                continue
-            if g.layout != torch.strided:
-                raise RuntimeError("AdamW: sparse gradients are not implemented")
-            if p.numel() != arena.sizes[i] or p.device != arena.device or not p.is_contiguous():
-                raise RuntimeError("AdamW: a parameter was reshaped or moved after its first step")
-            if g.dtype != p.dtype or g.device != arena.device or p.dtype not in _lib.TYPES:
-                raise RuntimeError(f"AdamW: a {p.dtype} parameter on {p.device} has a {g.dtype} gradient on {g.device}")
-            todo.append((i, p, g if g.is_contiguous() else g.contiguous()))
-        return todo
+        """What has a gradient, checked: launches of (indexes or None for all, their type, addresses, gradients)."""
+        params = group["params"]
+        grads = [p.grad for p in params]
+        if any(g is None for g in grads):
+            if self.capturable:
+                raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
+            which = [i for i, g in enumerate(grads) if g is not None]
+        else:
+            # the usual step: every parameter where it was and as it was, every gradient as the kernel takes it
+            where = [p.data_ptr() for p in params]
+            if (where == arena.where and [p.numel() for p in params] == arena.sizes
+                    and [g.numel() for g in grads] == arena.sizes and {g.dtype for g in grads} == arena.kinds and len(arena.kinds) == 1 and arena.together
+                    and not any([g.is_sparse for g in grads]) and all([g.is_contiguous() for g in grads])):
+                return [(None, params[0].dtype, where, grads)]
+            which = range(len(params))
+        some = {}
+        for i in which:
+            g = self._check(arena, i, params[i], grads[i])
+            idx, ps, gs = some.setdefault((params[i].dtype, arena.steps[i]), ([], [], []))
+            idx.append(i)
+            ps.append(params[i].data_ptr())
+            gs.append(g)
+        if len(which) == len(params):
+            arena.where, arena.kinds = [p.data_ptr() for p in params], {p.dtype for p in params}
+        return [(idx, dtype, ps, gs) for (dtype, _), (idx, ps, gs) in some.items()]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -191,21 +213,26 @@ class AdamW(torch.optim.Optimizer):
         if self.capturable:
             _lib.call("pin_adamw_scalars", _lib.ptr(arena.step_dev), _lib.ptr(lr_dev), *rates, wd, salt,
                       _lib.ptr(arena.scalars), stream)
-        buckets = {}
-        for i, p, g in todo:
-            if not self.capturable:
-                arena.steps[i] += 1
-            buckets.setdefault((p.dtype, arena.steps[i]), []).append((i, p, g))
-        for (dtype, t), some in buckets.items():
-            n = len(some)
-            ps = (ctypes.c_void_p * n)(*[p.data_ptr() for _, p, _ in some])
-            gs = (ctypes.c_void_p * n)(*[g.data_ptr() for _, _, g in some])
-            sizes = (ctypes.c_int64 * n)(*[arena.sizes[i] for i, _, _ in some])
-            offsets = (ctypes.c_int64 * n)(*[arena.offsets[i] for i, _, _ in some])
+        for idx, dtype, ps, gs in todo:
+            if idx is None:
+                n, sizes, offsets = len(ps), arena.c_sizes, arena.c_offsets
+            else:
+                n = len(idx)
+                sizes, offsets = (array("q", [x[i] for i in idx]) for x in (arena.sizes, arena.offsets))
+            t = arena.steps[0 if idx is None else idx[0]] + (0 if self.capturable else 1)
+            ps, gs = array("Q", ps), array("Q", [g.data_ptr() for g in gs])
             master = arena.master if dtype != torch.float32 else None
-            _lib.call("pin_adamw_step", ps, gs, sizes, offsets, n, _lib.TYPES[dtype], arena.bits, _lib.ptr(arena.m),
-                      _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total, *rates,
-                      float(group["eps"]), wd, t, salt, _lib.ptr(arena.scalars), stream)
+            _lib.call("pin_adamw_step", *(x.buffer_info()[0] for x in (ps, gs, sizes, offsets)), n, _lib.TYPES[dtype],
+                      arena.bits, _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total,
+                      *rates, float(group["eps"]), wd, t, salt, _lib.ptr(arena.scalars), stream)
+            if self.capturable:
+                continue
+            if idx is None:
+                arena.steps = [t] * n
+            else:
+                for i in idx:
+                    arena.steps[i] = t
+                arena.together = len(set(arena.steps)) == 1
 
     def offsets(self, group=0):
         """First element of each parameter of the group in the flat arrays."""
@@ -281,5 +308,6 @@ class AdamW(torch.optim.Optimizer):
             for key in want:
                 self.state[p][key].copy_(one[key])
             arena.steps[i] = int(one["step"])
+            arena.together = len(set(arena.steps)) == 1
             if arena.step_dev is not None:
                 arena.step_dev.fill_(arena.steps[i])
