@@ -952,7 +952,7 @@ int pin_mc_emit(const float* values, int64_t nx, int64_t ny, int64_t nz, float l
  * adjacent, rows row_stride elements apart) with p = softmax(row):
  *   log_prob [n]        log p of the row's label, 0 where the label is ignore_index
  *   entropy [n]         -sum p log p
- *   row_stats [n,2]     the row's maximum and log sum exp(row - maximum) (for the gradient; may be NULL)
+ *   row_stats [n,3]     what the gradient needs of the row, for pin_label_logprob_bwd (may be NULL)
  *   top_log_prob, top_index [n,top_k]   the top_k most probable classes, ties to the lower class
  * Classes at -inf have no share.  All of a row at -inf: log_prob -inf, entropy 0, classes 0..top_k-1
  * at -inf.  A NaN or +inf in a row: NaN, top_index -1.  A label outside [0, classes) that is not
@@ -967,13 +967,13 @@ int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t clas
 /*
  * pin_label_logprob_bwd -- d_logits [n, classes] (type `dtype`, contiguous) from the gradients of
  * log_prob, entropy and top_log_prob (each may be NULL: zero), recomputing the probabilities from
- * the logits and pin_label_logprob's row_stats, entropy and top_index.  An ignored label takes no
+ * the logits and pin_label_logprob's row_stats and top_index.  An ignored label takes no
  * part; a row without a distribution has gradient 0.
  */
 int pin_label_logprob_bwd(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
                           const int64_t* labels, int64_t ignore_index, int32_t top_k, const int64_t* top_index,
-                          const float* row_stats, const float* entropy, const float* d_log_prob,
-                          const float* d_entropy, const float* d_top, void* d_logits, void* stream);
+                          const float* row_stats, const float* d_log_prob, const float* d_entropy, const float* d_top,
+                          void* d_logits, void* stream);
 
 #define PIN_ADAMW_BLOCK 256              /* elements that share the exponents of an 8-bit moment */
 #define PIN_ADAMW_SCALARS_BYTES 64

@@ -230,7 +230,7 @@ _SIGS = {
     "pin_label_logprob": [c_void_p, i32, i64, i64, i64, c_void_p, i64, i32, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_void_p, c_void_p, c_void_p],
     "pin_label_logprob_bwd": [c_void_p, i32, i64, i64, i64, c_void_p, i64, i32, c_void_p, c_void_p, c_void_p, c_void_p,
-                              c_void_p, c_void_p, c_void_p, c_void_p],
+                              c_void_p, c_void_p, c_void_p],
     "pin_adamw_step": [c_void_p, c_void_p, c_void_p, c_void_p, i32, i32, i32, c_void_p, c_void_p, c_void_p,
                        c_void_p, i64, f64, f64, f64, f64, f64, i64, u32, c_void_p, c_void_p],
     "pin_adamw_scalars": [c_void_p, c_void_p, f64, f64, f64, f64, u32, c_void_p, c_void_p],
@@ -317,12 +317,20 @@ def stream(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index):
+    """stream() of a device by its number, as a whole number."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
 def on_device(device):
     """Context in which launches go to ``device`` (nothing to do where it is the current one)."""
-    device = torch.device(device)
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    index = device if isinstance(device, int) else torch.device(device).index
+    if index is None or index == torch.cuda.current_device():
+        return _HERE_ALREADY
+    return torch.cuda.device(index)
 
 
 def require_device(t):

@@ -245,10 +245,22 @@ __device__ __forceinline__ float row_entropy(const Row& r, float s, float t) {
 struct Out {
     float* log_prob;
     float* entropy;
-    float2* stats;      // may be NULL; maximum and log2 of the sum
+    float* stats;       // may be NULL; maximum, log2 of the sum, entropy
     float* top_lp;
     int64_t* top_idx;
 };
+
+__device__ __forceinline__ void put_row(const Out& o, const Row& r, int64_t row, float s, float t, float zy, int64_t y,
+                                        int64_t ignore, int64_t classes) {
+    const float h = row_entropy(r, s, t);
+    o.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
+    o.entropy[row] = h;
+    if (o.stats) {
+        o.stats[3 * row] = r.m;
+        o.stats[3 * row + 1] = r.ls;
+        o.stats[3 * row + 2] = h;
+    }
+}
 
 __device__ __forceinline__ void put_top(const Out& o, const Row& r, int64_t at, uint64_t key) {
     o.top_lp[at] = r.log_prob(key_value((uint32_t)(key >> 32)));
@@ -469,9 +481,7 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
     t = wave_sum(t);
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);   // s >= 1 unless there is nothing
     if (lane == 0) {
-        out.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
-        out.entropy[row] = row_entropy(r, s, t);
-        if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+        put_row(out, r, row, s, t, zy, y, ignore, classes);
         s_c.n_gt = s_c.n_eq = 0;
     }
     if (!TOP) return;
@@ -547,9 +557,7 @@ k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t r
     }
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
     const int64_t y = labels[row];
-    out.log_prob[row] = label_log_prob(r, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
-    out.entropy[row] = row_entropy(r, s, t);
-    if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+    put_row(out, r, row, s, t, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
 }
 
 // The parts' sums taken to the row's maximum (one lane per part, every wave alike).
@@ -566,9 +574,7 @@ __device__ __forceinline__ Row join_sums(const float4* __restrict__ sums, const 
     const float s = wave_sum(f * p.y), t = wave_sum(f * fmaf(p.y, x, p.z));
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
     if (threadIdx.x == 0) {
-        out.log_prob[row] = label_log_prob(r, zy, y, ignore, classes);
-        out.entropy[row] = row_entropy(r, s, t);
-        if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+        put_row(out, r, row, s, t, zy, y, ignore, classes);
     }
     return r;
 }
@@ -777,9 +783,7 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
     if (tid == 0) {
         const int64_t y = labels[row];
-        out.log_prob[row] = label_log_prob(r, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
-        out.entropy[row] = row_entropy(r, s, t);
-        if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+        put_row(out, r, row, s, t, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
     }
     if (k == 0) return;
     const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
@@ -825,9 +829,7 @@ k_label_small(const typename T::type* __restrict__ logits, int64_t n, int classe
         t = fmaf(e, x, t);
     }
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
-    out.log_prob[row] = label_log_prob(r, y >= 0 && y < classes ? z[y] : 0.f, y, ignore, classes);
-    out.entropy[row] = row_entropy(r, s, t);
-    if (out.stats) out.stats[row] = make_float2(r.m, r.ls);
+    put_row(out, r, row, s, t, y >= 0 && y < classes ? z[y] : 0.f, y, ignore, classes);
     float last = kInf;
     int last_j = -1;
     for (int i = 0; i < k; ++i) {   // the largest behind the last one, the first of equal ones
@@ -855,13 +857,13 @@ struct Grads {
 struct RowGrad {
     Row r;
     float lp, h, gh, g;   // the label's own term, H log2 e, g_H ln 2, G
-    __device__ __forceinline__ RowGrad(const float2* stats, const float* entropy, const Grads& u, int64_t row, int64_t y,
-                                       int64_t ignore, int64_t classes, int k)
-        : r(stats[row].x) {
-        r.ls = stats[row].y;
+    __device__ __forceinline__ RowGrad(const float* stats, const Grads& u, int64_t row, int64_t y, int64_t ignore,
+                                       int64_t classes, int k)
+        : r(stats[3 * row]) {
+        r.ls = stats[3 * row + 1];
         lp = u.lp && y != ignore ? (y < 0 || y >= classes ? NAN : u.lp[row]) : 0.f;
         gh = u.ent ? u.ent[row] * kLn2 : 0.f;
-        h = entropy[row] * kL;
+        h = stats[3 * row + 2] * kL;
         g = lp;
         if (u.top)
             for (int i = 0; i < k; ++i) g += u.top[row * k + i];
@@ -879,7 +881,7 @@ template <class T, int LANES>
 __global__ void __launch_bounds__(256)
 k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int64_t classes, int64_t row_stride,
             const int64_t* __restrict__ labels, int64_t ignore, int k, const int64_t* __restrict__ top_idx,
-            const float2* __restrict__ stats, const float* __restrict__ entropy, Grads u, int64_t part,
+            const float* __restrict__ stats, Grads u, int64_t part,
             typename T::type* __restrict__ out) {
     constexpr int V = T::N;
     const int lane = threadIdx.x % LANES;
@@ -890,7 +892,7 @@ k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int64_t clas
     const typename T::type* z = logits + (on ? row : 0) * row_stride;
     typename T::type* o = out + (on ? row : 0) * classes;
     const int64_t y = on ? labels[row] : ignore;
-    const RowGrad d(stats, entropy, u, on ? row : 0, y, ignore, classes, k);
+    const RowGrad d(stats, u, on ? row : 0, y, ignore, classes, k);
     const bool plain = !d.r.far && !d.r.bad() && !d.r.dead();
     if (on) {
         for (int64_t j = first + lane * V; j < end; j += LANES * V) {
@@ -930,7 +932,7 @@ template <class T, int ROWS>
 __global__ void __launch_bounds__(ROWS)
 k_label_bwd_small(const typename T::type* __restrict__ logits, int64_t n, int classes, uint32_t magic, int64_t row_stride,
                   const int64_t* __restrict__ labels, int64_t ignore, int k, const int64_t* __restrict__ top_idx,
-                  const float2* __restrict__ stats, const float* __restrict__ entropy, Grads u,
+                  const float* __restrict__ stats, Grads u,
                   typename T::type* __restrict__ out) {
     extern __shared__ float s_z[];
     const int64_t row0 = (int64_t)blockIdx.x * ROWS;
@@ -939,7 +941,7 @@ k_label_bwd_small(const typename T::type* __restrict__ logits, int64_t n, int cl
     const int pitch = classes | 1;
     if ((int)threadIdx.x < rows) {
         const int64_t row = row0 + threadIdx.x, y = labels[row];
-        const RowGrad d(stats, entropy, u, row, y, ignore, classes, k);
+        const RowGrad d(stats, u, row, y, ignore, classes, k);
         float* z = s_z + threadIdx.x * pitch;
         for (int j = 0; j < classes; ++j) z[j] = d.value(z[j]);
         if (!d.r.dead()) {
@@ -1076,8 +1078,7 @@ int run_forward(const Call& a) {
 }
 
 template <class T>
-int run_backward(const Call& a, const int64_t* top_idx, const float2* stats, const float* entropy, const Grads& u,
-                 void* d_logits) {
+int run_backward(const Call& a, const int64_t* top_idx, const float* stats, const Grads& u, void* d_logits) {
     typename T::type* o = (typename T::type*)d_logits;
     const typename T::type* z = (const typename T::type*)a.logits;
     if (a.classes <= kSmall) {
@@ -1088,11 +1089,11 @@ int run_backward(const Call& a, const int64_t* top_idx, const float2* stats, con
         if (rows == 256)
             hipLaunchKernelGGL((k_label_bwd_small<T, 256>), dim3((unsigned)blocks), dim3(256), lds, a.st, z, a.n,
                                (int)a.classes, magic_of(a.classes), a.row_stride, a.labels, a.ignore, a.k, top_idx, stats,
-                               entropy, u, o);
+                               u, o);
         else
             hipLaunchKernelGGL((k_label_bwd_small<T, 128>), dim3((unsigned)blocks), dim3(128), lds, a.st, z, a.n,
                                (int)a.classes, magic_of(a.classes), a.row_stride, a.labels, a.ignore, a.k, top_idx, stats,
-                               entropy, u, o);
+                               u, o);
         return launch_status();
     }
     const int lanes = a.classes <= 16 * T::N * 4 ? 16 : a.classes <= 64 * T::N * 8 ? 64 : 256;
@@ -1106,13 +1107,13 @@ int run_backward(const Call& a, const int64_t* top_idx, const float2* stats, con
     const dim3 grid((unsigned)blocks, (unsigned)parts);
     if (lanes == 16)
         hipLaunchKernelGGL((k_label_bwd<T, 16>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
-                           a.ignore, a.k, top_idx, stats, entropy, u, part, o);
+                           a.ignore, a.k, top_idx, stats, u, part, o);
     else if (lanes == 64)
         hipLaunchKernelGGL((k_label_bwd<T, 64>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
-                           a.ignore, a.k, top_idx, stats, entropy, u, part, o);
+                           a.ignore, a.k, top_idx, stats, u, part, o);
     else
         hipLaunchKernelGGL((k_label_bwd<T, 256>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
-                           a.ignore, a.k, top_idx, stats, entropy, u, part, o);
+                           a.ignore, a.k, top_idx, stats, u, part, o);
     return launch_status();
 }
 
@@ -1134,28 +1135,27 @@ int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t clas
                       float* row_stats, float* top_log_prob, int64_t* top_index, void* workspace, void* stream) {
     if (bad_args(logits, dtype, n, classes, row_stride, labels, top_k)) return PIN_ERR_ARG;
     if (n == 0) return PIN_OK;
-    if (!log_prob || !entropy || (top_k > 0 && (!top_log_prob || !top_index)) || ((uintptr_t)row_stats & 7))
+    if (!log_prob || !entropy || (top_k > 0 && (!top_log_prob || !top_index)))
         return PIN_ERR_ARG;
     const Call a{logits, n, classes, row_stride, labels, ignore_index, (int)top_k,
-                 Out{log_prob, entropy, (float2*)row_stats, top_log_prob, top_index}, workspace, as_stream(stream)};
+                 Out{log_prob, entropy, row_stats, top_log_prob, top_index}, workspace, as_stream(stream)};
     return dtype == PIN_TYPE_F32 ? run_forward<F32>(a) : dtype == PIN_TYPE_F16 ? run_forward<F16>(a) : run_forward<BF16>(a);
 }
 
 int pin_label_logprob_bwd(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
                           const int64_t* labels, int64_t ignore_index, int32_t top_k, const int64_t* top_index,
-                          const float* row_stats, const float* entropy, const float* d_log_prob,
-                          const float* d_entropy, const float* d_top, void* d_logits, void* stream) {
+                          const float* row_stats, const float* d_log_prob, const float* d_entropy, const float* d_top,
+                          void* d_logits, void* stream) {
     if (bad_args(logits, dtype, n, classes, row_stride, labels, top_k)) return PIN_ERR_ARG;
     if (n == 0) return PIN_OK;
-    if (!row_stats || ((uintptr_t)row_stats & 7) || !entropy || !d_logits || (d_top && top_k > 0 && !top_index) ||
+    if (!row_stats || !d_logits || (d_top && top_k > 0 && !top_index) ||
         ((uintptr_t)d_logits & (dtype == PIN_TYPE_F32 ? 3 : 1)))
         return PIN_ERR_ARG;
     const Call a{logits, n, classes, row_stride, labels, ignore_index, (int)top_k, Out{}, nullptr, as_stream(stream)};
     const Grads u{d_log_prob, d_entropy, top_k > 0 ? d_top : nullptr};
-    const float2* st = (const float2*)row_stats;
-    return dtype == PIN_TYPE_F32   ? run_backward<F32>(a, top_index, st, entropy, u, d_logits)
-           : dtype == PIN_TYPE_F16 ? run_backward<F16>(a, top_index, st, entropy, u, d_logits)
-                                   : run_backward<BF16>(a, top_index, st, entropy, u, d_logits);
+    return dtype == PIN_TYPE_F32   ? run_backward<F32>(a, top_index, row_stats, u, d_logits)
+           : dtype == PIN_TYPE_F16 ? run_backward<F16>(a, top_index, row_stats, u, d_logits)
+                                   : run_backward<BF16>(a, top_index, row_stats, u, d_logits);
 }
 
 }  // extern "C"

@@ -16,46 +16,64 @@ LabelLogProbs = namedtuple("LabelLogProbs", ["log_prob", "entropy", "top_log_pro
 
 
 def _forward(z, y, k, ignore, want_stats):
+    """log_prob [n], entropy [n], row statistics [n, 3] or None, top_log_prob and top_index [n, k] or None, of the
+    rows z [n, C]."""
     n, c = z.shape
     dev = z.device
-    # one allocation for what is f32: the two columns, the statistics, the alternatives
-    buf = torch.empty((2 * n * (1 + want_stats) + n * k,), dtype=torch.float32, device=dev)
-    at = 2 * n * (1 + want_stats)
-    lp, ent, stats, tlp = buf[:n], buf[n:2 * n], buf[2 * n:at] if want_stats else None, buf[at:].view(n, k)
-    tidx = torch.empty((n, k), dtype=torch.int64, device=dev)
+    lp = torch.empty((n,), dtype=torch.float32, device=dev)
+    ent = torch.empty((n,), dtype=torch.float32, device=dev)
+    stats = torch.empty((n, 3), dtype=torch.float32, device=dev) if want_stats else None
+    tlp = torch.empty((n, k), dtype=torch.float32, device=dev) if k else None
+    tidx = torch.empty((n, k), dtype=torch.int64, device=dev) if k else None
     dt = _lib.TYPES[z.dtype]
-    base = buf.data_ptr()
-    with _lib.on_device(dev):
-        need = _lib.fn("pin_label_logprob_workspace_bytes")(n, c, dt, k)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-        _lib.call("pin_label_logprob", z.data_ptr(), dt, n, c, z.stride(0), y.data_ptr(), ignore, k, base, base + 4 * n,
-                  base + 8 * n if want_stats else None, base + 4 * at if k else None, tidx.data_ptr() if k else None,
-                  None if ws is None else ws.data_ptr(), _lib.stream(dev))
+    need = _lib.fn("pin_label_logprob_workspace_bytes")(n, c, dt, k)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
+    _lib.call("pin_label_logprob", z.data_ptr(), dt, n, c, z.stride(0), y.data_ptr(), ignore, k, lp.data_ptr(),
+              ent.data_ptr(), stats.data_ptr() if want_stats else None, tlp.data_ptr() if k else None,
+              tidx.data_ptr() if k else None, None if ws is None else ws.data_ptr(), _lib.raw_stream(z.get_device()))
     return lp, ent, stats, tlp, tidx
 
 
+def _f32(g):
+    """An upstream gradient as the kernel takes it."""
+    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+
+
+def _backward(ctx, g_lp, g_ent, g_top=None, _=None):
+    z, y, *top = ctx.saved_tensors
+    n, c = z.shape
+    k = top[0].shape[1] if top else 0
+    g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
+    dz = z.new_empty((n, c))
+    # (autograd runs this on the logits' device and the forward's stream)
+    _lib.call("pin_label_logprob_bwd", z.data_ptr(), _lib.TYPES[z.dtype], n, c, z.stride(0), y.data_ptr(), ctx.ignore, k,
+              top[0].data_ptr() if top else None, ctx.stats.data_ptr(), None if g_lp is None else g_lp.data_ptr(),
+              None if g_ent is None else g_ent.data_ptr(), None if g_top is None else g_top.data_ptr(), dz.data_ptr(),
+              _lib.raw_stream(z.get_device()))
+    return dz, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _LabelLogProbFn(torch.autograd.Function):
+    """(log_prob, entropy), and with k > 0 (top_log_prob, top_index)."""
+
     @staticmethod
     def forward(ctx, z, y, k, ignore):
         ctx.set_materialize_grads(False)
         lp, ent, stats, tlp, tidx = _forward(z, y, k, ignore, True)
-        ctx.save_for_backward(z, y, stats, ent, tidx)
-        ctx.ignore = ignore
+        ctx.stats, ctx.ignore = stats, ignore
+        if k == 0:
+            ctx.save_for_backward(z, y)
+            return lp, ent
+        ctx.save_for_backward(z, y, tidx)
         ctx.mark_non_differentiable(tidx)
         return lp, ent, tlp, tidx
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _):
-        z, y, stats, ent, tidx = ctx.saved_tensors
-        n, c = z.shape
-        g_lp, g_ent, g_top = (None if g is None else g.to(torch.float32).contiguous() for g in (g_lp, g_ent, g_top))
-        dz = torch.empty((n, c), dtype=z.dtype, device=z.device)
-        with _lib.on_device(z.device):
-            _lib.call("pin_label_logprob_bwd", z.data_ptr(), _lib.TYPES[z.dtype], n, c, z.stride(0), _lib.ptr(y),
-                      ctx.ignore, tidx.shape[1], _lib.ptr(tidx), _lib.ptr(stats), _lib.ptr(ent), _lib.ptr(g_lp),
-                      _lib.ptr(g_ent), _lib.ptr(g_top), _lib.ptr(dz), _lib.stream(z.device))
-        return dz, None, None, None
+    def backward(ctx, *g):
+        return _backward_once(ctx, *g) if torch.is_grad_enabled() else _backward(ctx, *g)
 
 
 def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, ignore_index: int = -100):
@@ -84,18 +102,22 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
     k = int(top_k)
     if not 0 <= k <= min(c, _lib.LABEL_TOP_MAX):
         raise ValueError(f"label_log_probs: top_k must be 0 to min(classes, {_lib.LABEL_TOP_MAX}) (got {top_k})")
-    lead = logits.shape[:-1]
-    n = 1
-    for s in lead:
-        n *= s
-    z = logits.reshape(n, c)
-    if c > 1 and z.stride(1) != 1 or z.stride(0) < 0:
+    z, y = logits, labels
+    if logits.dim() != 2:
+        z, y = logits.reshape(labels.numel(), c), labels.reshape(-1)
+    if c > 1 and z.stride(1) != 1:
         z = z.contiguous()
-    y = labels.reshape(n).to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, ent, tlp, tidx = _LabelLogProbFn.apply(z, y, k, int(ignore_index))
-    else:
-        lp, ent, _, tlp, tidx = _forward(z.detach(), y, k, int(ignore_index), False)
-    if len(lead) == 1:
-        return LabelLogProbs(lp, ent, tlp, tidx)
-    return LabelLogProbs(lp.view(lead), ent.view(lead), tlp.view(lead + (k,)), tidx.view(lead + (k,)))
+    if y.dtype != torch.int64 or not y.is_contiguous():
+        y = y.to(torch.int64).contiguous()
+    with _lib.on_device(z.get_device()):
+        if torch.is_grad_enabled() and logits.requires_grad:
+            lp, ent, *top = _LabelLogProbFn.apply(z, y, k, int(ignore_index))
+        else:
+            lp, ent, _, *top = _forward(z, y, k, int(ignore_index), False)
+    if k == 0:
+        top = lp.new_empty((lp.shape[0], 0)), y.new_empty((lp.shape[0], 0))
+    tlp, tidx = top
+    if logits.dim() != 2:
+        lead = labels.shape
+        lp, ent, tlp, tidx = lp.view(lead), ent.view(lead), tlp.view(lead + (k,)), tidx.view(lead + (k,))
+    return LabelLogProbs(lp, ent, tlp, tidx)

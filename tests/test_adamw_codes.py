@@ -80,9 +80,9 @@ def test_argument_errors_before_any_device_work():
                 dict(stride=-1), dict(labels=None), dict(k=11), dict(k=33, c=100), dict(k=-1), dict(lp=None),
                 dict(ent=None), dict(top=None), dict(idx=None), dict(logits=ctypes.c_void_p(4098))):
         assert logprob(**bad) == -1, bad
-    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, ok, None, ok, ok, ok, ok, ok, None) == -1
-    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, None, ok, ok, ok, ok, ok, ok, None) == -1
-    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, ok, ok, ok, ok, ok, ok, None, None) == -1
+    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, ok, None, ok, ok, ok, ok, None) == -1
+    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, None, ok, ok, ok, ok, ok, None) == -1
+    assert lib.pin_label_logprob_bwd(ok, 0, 4, 10, 10, ok, -100, 2, ok, ok, ok, ok, ok, None, None) == -1
 
     def adamw(ps=(4096, 8192), gs=(4096, 8192), sizes=(300, 5), offsets=(0, 512), dtype=0, bits=8, m=ok, v=ok, e=ok, w=None,
               total=768, lr=0.1, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, step=1, scalars=None):
