@@ -92,35 +92,38 @@ __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half(v); }
 __device__ __forceinline__ void from_f32(float v, __hip_bfloat16& o) { o = __float2bfloat16(v); }
 
-// four consecutive elements, vector accesses where all are there and the address allows them
+// four consecutive elements in one access, or (where they are not all there, or not aligned) one by one;
+// which of the two is the same for the wave
 template <class T>
 struct alignas(4 * sizeof(T)) Four {
     T v[4];
 };
 template <class T>
-__device__ __forceinline__ void load4(const T* __restrict__ p, int64_t i, int64_t n, float (&o)[4]) {
-    const T* q = p + i;
-    if (i + 4 <= n && ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0) {
-        const Four<T> f = *(const Four<T>*)q;
+__device__ __forceinline__ bool aligned4(const T* p) {
+    return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
+}
+template <class T>
+__device__ __forceinline__ void load4(const T* __restrict__ p, int64_t i, int64_t n, bool whole, float (&o)[4]) {
+    if (whole) {
+        const Four<T> f = *(const Four<T>*)(p + i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = to_f32(f.v[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = i + k < n ? to_f32(q[k]) : 0.f;
+        for (int k = 0; k < 4; ++k) o[k] = i + k < n ? to_f32(p[i + k]) : 0.f;
     }
 }
 template <class T>
-__device__ __forceinline__ void store4(T* __restrict__ p, int64_t i, int64_t n, const float (&v)[4]) {
-    T* q = p + i;
-    if (i + 4 <= n && ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0) {
+__device__ __forceinline__ void store4(T* __restrict__ p, int64_t i, int64_t n, bool whole, const float (&v)[4]) {
+    if (whole) {
         Four<T> f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) from_f32(v[k], f.v[k]);
-        *(Four<T>*)q = f;
+        *(Four<T>*)(p + i) = f;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) from_f32(v[k], q[k]);
+            if (i + k < n) from_f32(v[k], p[i + k]);
     }
 }
 
@@ -131,6 +134,8 @@ __device__ __forceinline__ int find_tensor(const AdamwTable& t, uint32_t chunk) 
     const uint32_t b = lane + 64 < t.count ? t.chunk0[lane + 64] : ~0u;
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(a <= chunk)) + __popcll(__ballot(b <= chunk)) - 1);
 }
+
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 __device__ __forceinline__ float adamw_update(float p, float m, float v, float eps, const AdamwScalars& a) {
     p = p * a.decay;
@@ -143,14 +148,17 @@ k_adamw32(AdamwTable t, float* __restrict__ m_, float* __restrict__ v_, float* _
           AdamwScalars host, const AdamwScalars* __restrict__ dev) {
     const AdamwScalars a = dev ? *dev : host;
     const int k = find_tensor(t, blockIdx.x);
-    const int64_t i = (int64_t)(blockIdx.x - t.chunk0[k]) * kChunk + threadIdx.x * 4;
     const int64_t n = t.n[k];
+    const int64_t i0 = (int64_t)(blockIdx.x - t.chunk0[k]) * kChunk + wave_of() * kGroup, i = i0 + (threadIdx.x & 63) * 4;
     if (i >= n) return;
     const int64_t s = (int64_t)t.block0[k] * kGroup + i;   // 16-byte aligned, padded to whole blocks
+    const T* gp = (const T*)t.g[k];
+    T* pp = (T*)t.p[k];
+    const bool all = i0 + kGroup <= n;
     float p[4], g[4];
-    load4((const T*)t.g[k], i, n, g);
-    if (MASTER) load4(w_ + (s - i), i, n, p);
-    else load4((const T*)t.p[k], i, n, p);
+    load4(gp, i, n, all && aligned4(gp), g);
+    if (MASTER) load4(w_ + (s - i), i, n, all, p);
+    else load4((const T*)pp, i, n, all && aligned4(pp), p);
     float4 m4 = *(float4*)(m_ + s), v4 = *(float4*)(v_ + s);
     float m[4] = {m4.x, m4.y, m4.z, m4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
     const float b1 = (float)a.b1, b2 = (float)a.b2, c1 = (float)a.c1, c2 = (float)a.c2;
@@ -162,8 +170,8 @@ k_adamw32(AdamwTable t, float* __restrict__ m_, float* __restrict__ v_, float* _
     }
     *(float4*)(m_ + s) = make_float4(m[0], m[1], m[2], m[3]);
     *(float4*)(v_ + s) = make_float4(v[0], v[1], v[2], v[3]);
-    if (MASTER) store4(w_ + (s - i), i, n, p);
-    store4((T*)t.p[k], i, n, p);
+    if (MASTER) store4(w_ + (s - i), i, n, all, p);
+    store4(pp, i, n, all && aligned4(pp), p);
 }
 
 __device__ __forceinline__ double pow2(int e) { return __longlong_as_double((long long)(e + 1023) << 52); }
@@ -184,12 +192,19 @@ __device__ __forceinline__ float decode_v(uint32_t c) {
 
 __device__ __forceinline__ uint32_t hi32(double x) { return (uint32_t)((uint64_t)__double_as_longlong(x) >> 32); }
 
+template <int CTRL>
+__device__ __forceinline__ int max_of_lanes(int v) {
+    const int b = __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
+    return b > v ? b : v;
+}
+// the largest of the wave's values
 __device__ __forceinline__ int wave_max(int v) {
-    for (int o = 32; o; o >>= 1) {
-        const int b = __shfl_xor(v, o);
-        v = b > v ? b : v;
-    }
-    return v;
+    v = max_of_lanes<0xB1>(v);    // lanes ^ 1
+    v = max_of_lanes<0x4E>(v);    // lanes ^ 2
+    v = max_of_lanes<0x141>(v);   // the other half of 8
+    v = max_of_lanes<0x140>(v);   // the other half of 16
+    const int a = max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+    return max(a, max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 // exponent of the largest finite of a block's values, four per lane
@@ -200,7 +215,7 @@ __device__ __forceinline__ int block_exponent(const double (&x)[4]) {
         const int a = (int)(hi32(x[j]) & 0x7FFFFFFF);
         h = a < 0x7FF00000 && a > h ? a : h;
     }
-    const int e = (__builtin_amdgcn_readfirstlane(wave_max(h)) >> 20) - 1023;
+    const int e = (wave_max(h) >> 20) - 1023;
     return e < kLeast ? kLeast : e;
 }
 
@@ -217,6 +232,10 @@ __device__ __forceinline__ uint32_t encode_v(double x, int e, uint32_t dither) {
     return h >= 0x7FF00000u ? 0xFF : (uint32_t)c;
 }
 
+// One wave per block of 256 elements, four per lane.  The parameter's step is taken in f32 from the new
+// averages before they are coded, numerator and denominator over the power of two of the block's largest
+// square root: they are normal numbers at any size of the gradients, which the hardware's square root and
+// reciprocal (one unit in the last place each) need.
 template <class T, bool MASTER>
 __global__ void __launch_bounds__(kBlock)
 k_adamw8(AdamwTable t, uint32_t* __restrict__ m_, uint32_t* __restrict__ v_, short2* __restrict__ e_,
@@ -224,41 +243,46 @@ k_adamw8(AdamwTable t, uint32_t* __restrict__ m_, uint32_t* __restrict__ v_, sho
     const AdamwScalars a = dev ? *dev : host;
     const int k = find_tensor(t, blockIdx.x);
     const int64_t n = t.n[k];
-    const int64_t chunk = (int64_t)(blockIdx.x - t.chunk0[k]) * kChunk;
+    const int64_t i0 = (int64_t)(blockIdx.x - t.chunk0[k]) * kChunk + wave_of() * kGroup;
+    if (i0 >= n) return;
     const int lane = threadIdx.x & 63;
-    for (int64_t i0 = chunk + (threadIdx.x >> 6) * kGroup; i0 < n && i0 < chunk + kChunk; i0 += kBlock / 64 * kGroup) {
-        const int64_t b = (int64_t)t.block0[k] + i0 / kGroup;
-        const int64_t i = i0 + lane * 4, s = b * kGroup + lane * 4;
-        float p[4], g[4], cm[4];
-        load4((const T*)t.g[k], i, n, g);
-        if (MASTER) load4(w_ + (s - i), i, n, p);
-        else load4((const T*)t.p[k], i, n, p);
-        const uint32_t um = m_[s / 4], uv = v_[s / 4];
-        const short2 e = e_[b];
-        decode_m(um, cm);
-        const double sm = pow2(e.x - 7) * a.b1, sv = pow2(e.y) * a.b2;
-        double m[4], v[4];
+    const int64_t b = (int64_t)t.block0[k] + i0 / kGroup;
+    const int64_t i = i0 + lane * 4, s = b * kGroup + lane * 4;
+    const T* gp = (const T*)t.g[k];
+    T* pp = (T*)t.p[k];
+    const bool all = i0 + kGroup <= n, pa = all && aligned4(pp);
+    float p[4], g[4], cm[4];
+    load4(gp, i, n, all && aligned4(gp), g);
+    if (MASTER) load4(w_ + (s - i), i, n, all, p);
+    else load4((const T*)pp, i, n, pa, p);
+    const uint32_t um = m_[s / 4], uv = v_[s / 4];
+    const short2 e = e_[b];
+    decode_m(um, cm);
+    const double sm = pow2(e.x - 7) * a.b1, sv = pow2(e.y) * a.b2;
+    double m[4], v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double d = (double)g[j];
-            m[j] = (double)cm[j] * sm + d * a.c1;
-            v[j] = (double)decode_v((uv >> 8 * j) & 0xFF) * sv + d * d * a.c2;
-            p[j] = adamw_update(p[j], (float)m[j], (float)v[j], eps, a);
-        }
-        const int em = block_exponent(m), ev = block_exponent(v);
-        uint32_t om = 0, ov = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t h = mix32(a.key + ((uint32_t)s + j) * kMix3);
-            om |= encode_m(m[j], em, h & 0x1FFFF) << 8 * j;
-            ov |= encode_v(v[j], ev, h >> 15) << 8 * j;
-        }
-        m_[s / 4] = om;
-        v_[s / 4] = ov;
-        if (lane == 0) e_[b] = make_short2((short)em, (short)ev);
-        if (MASTER) store4(w_ + (s - i), i, n, p);
-        store4((T*)t.p[k], i, n, p);
+    for (int j = 0; j < 4; ++j) {
+        const double d = (double)g[j];
+        m[j] = (double)cm[j] * sm + d * a.c1;
+        v[j] = (double)decode_v((uv >> 8 * j) & 0xFF) * sv + d * d * a.c2;
     }
+    const int em = block_exponent(m), ev = block_exponent(v), half = ev >> 1;
+    const double down = pow2(-half), down2 = pow2(-2 * half);
+    const float inv = 1.f / a.bc2_sqrt, eps_down = (float)((double)eps * down);
+    uint32_t om = 0, ov = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float den = fmaf(__builtin_amdgcn_sqrtf((float)(v[j] * down2)), inv, eps_down);
+        p[j] = p[j] * a.decay - a.step_size * ((float)(m[j] * down) * __builtin_amdgcn_rcpf(den));
+        const uint32_t h = mix32(a.key + ((uint32_t)s + j) * kMix3);
+        om |= encode_m(m[j], em, h & 0x1FFFF) << 8 * j;
+        ov |= encode_v(v[j], ev, h >> 15) << 8 * j;
+    }
+    m_[s / 4] = om;
+    v_[s / 4] = ov;
+    if (lane == 0) e_[b] = make_short2((short)em, (short)ev);
+    if (MASTER) store4(w_ + (s - i), i, n, all, p);
+    store4(pp, i, n, pa, p);
 }
 
 __global__ void __launch_bounds__(kBlock)

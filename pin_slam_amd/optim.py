@@ -17,6 +17,8 @@ import torch
 
 from . import _lib
 
+_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_dtype = torch.Tensor.dtype.__get__
 _SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
 
@@ -50,6 +52,7 @@ class _Arena:
                 self.master[a:a + n] = p.detach().reshape(-1)
         self.steps = [0] * len(params)
         self.together = True              # all of them are the same
+        self.held = None
         self.where, self.kinds = None, set()   # the parameters as they were last checked one by one
         self.c_sizes, self.c_offsets = array("q", self.sizes), array("q", self.offsets)
         # a step that a graph may replay counts on the device, all of the group's parameters together
@@ -155,28 +158,35 @@ class AdamW(torch.optim.Optimizer):
         return g if g.is_contiguous() else g.contiguous()
 
     def _gather(self, arena, group):
-        """What has a gradient, checked: launches of (indexes or None for all, their type, addresses, gradients)."""
+        """What has a gradient, checked: launches of (indexes or None for all, their type, addresses of the parameters and
+        of the gradients)."""
         params = group["params"]
         grads = [p.grad for p in params]
-        if any(g is None for g in grads):
+        if type(None) in set(map(type, grads)):
             if self.capturable:
                 raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
             which = [i for i, g in enumerate(grads) if g is not None]
         else:
-            # the usual step: every parameter where it was and as it was, every gradient as the kernel takes it
-            where = [p.data_ptr() for p in params]
-            if (where == arena.where and [p.numel() for p in params] == arena.sizes
-                    and [g.numel() for g in grads] == arena.sizes and {g.dtype for g in grads} == arena.kinds and len(arena.kinds) == 1 and arena.together
-                    and not any([g.is_sparse for g in grads]) and all([g.is_contiguous() for g in grads])):
-                return [(None, params[0].dtype, where, grads)]
+            # the usual step: every parameter where it was and as it was, every gradient as the kernel takes it.  One
+            # pass per property: for many tensors this is the step's cost on the host.
+            where = list(map(_ptr, params))
+            try:
+                if (where == arena.where and arena.together and list(map(_numel, params)) == arena.sizes
+                        and list(map(_numel, grads)) == arena.sizes and set(map(_dtype, grads)) == arena.kinds
+                        and len(arena.kinds) == 1 and all(map(_contiguous, grads))):
+                    return [(None, params[0].dtype, where, list(map(_ptr, grads)))]
+            except RuntimeError:   # a sparse one has no contiguity and no address
+                pass
             which = range(len(params))
         some = {}
+        held = arena.held = []   # copies made here live until the step is on its way
         for i in which:
             g = self._check(arena, i, params[i], grads[i])
             idx, ps, gs = some.setdefault((params[i].dtype, arena.steps[i]), ([], [], []))
             idx.append(i)
             ps.append(params[i].data_ptr())
-            gs.append(g)
+            gs.append(g.data_ptr())
+            held.append(g)
         if len(which) == len(params):
             arena.where, arena.kinds = [p.data_ptr() for p in params], {p.dtype for p in params}
         return [(idx, dtype, ps, gs) for (dtype, _), (idx, ps, gs) in some.items()]
@@ -220,7 +230,7 @@ class AdamW(torch.optim.Optimizer):
                 n = len(idx)
                 sizes, offsets = (array("q", [x[i] for i in idx]) for x in (arena.sizes, arena.offsets))
             t = arena.steps[0 if idx is None else idx[0]] + (0 if self.capturable else 1)
-            ps, gs = array("Q", ps), array("Q", [g.data_ptr() for g in gs])
+            ps, gs = array("Q", ps), array("Q", gs)
             master = arena.master if dtype != torch.float32 else None
             _lib.call("pin_adamw_step", *(x.buffer_info()[0] for x in (ps, gs, sizes, offsets)), n, _lib.TYPES[dtype],
                       arena.bits, _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total,
@@ -233,6 +243,7 @@ class AdamW(torch.optim.Optimizer):
                 for i in idx:
                     arena.steps[i] = t
                 arena.together = len(set(arena.steps)) == 1
+        arena.held = None
 
     def offsets(self, group=0):
         """First element of each parameter of the group in the flat arrays."""
