@@ -919,16 +919,15 @@ struct Grads {
 struct RowGrad {
     Row r;
     float lp, h, gh, g;   // the label's own term, H log2 e, g_H ln 2, G
+    // top: the sum of the alternatives' upstream gradients
     __device__ __forceinline__ RowGrad(const float* stats, const Grads& u, int64_t row, int64_t y, int64_t ignore,
-                                       int64_t classes, int k)
+                                       int64_t classes, float top)
         : r(stats[3 * row]) {
         r.ls = stats[3 * row + 1];
         lp = u.lp && y != ignore ? (y < 0 || y >= classes ? NAN : u.lp[row]) : 0.f;
         gh = u.ent ? u.ent[row] * kLn2 : 0.f;
         h = stats[3 * row + 2] * kL;
-        g = lp;
-        if (u.top)
-            for (int i = 0; i < k; ++i) g += u.top[row * k + i];
+        g = lp + top;
     }
     // without the given terms
     __device__ __forceinline__ float dz(float z) const {
@@ -938,56 +937,74 @@ struct RowGrad {
     __device__ __forceinline__ float value(float z) const { return r.dead() ? 0.f : r.bad() ? NAN : dz(z); }
 };
 
-// LANES threads per row (a part of it, gridDim.y of them), vectors of 16 bytes
+template <int LANES>
+__device__ __forceinline__ float sum_of(float v) {   // over a row's lanes, of more than 64 over the wave's
+    return LANES == 16 ? __uint_as_float(rows_of_16(__float_as_uint(v), AddF())) : wave_sum(v);
+}
+
+// LANES threads per row, or per part of it (gridDim.y of them).  The vectors are the gradient's, aligned; the
+// logits' may lie otherwise.
 template <class T, int LANES>
 __global__ void __launch_bounds__(256)
-k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int64_t classes, int64_t row_stride,
+k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int classes, int64_t row_stride,
             const int64_t* __restrict__ labels, int64_t ignore, int k, const int64_t* __restrict__ top_idx,
-            const float* __restrict__ stats, Grads u, int64_t part,
-            typename T::type* __restrict__ out) {
-    constexpr int V = T::N;
+            const float* __restrict__ stats, Grads u, int part, typename T::type* __restrict__ out) {
+    constexpr int V = T::N, B = 4;
     const int lane = threadIdx.x % LANES;
     const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const bool on = row < n;
-    const int64_t first = blockIdx.y * part;
-    const int64_t end = first + part < classes ? first + part : classes;
     const typename T::type* z = logits + (on ? row : 0) * row_stride;
     typename T::type* o = out + (on ? row : 0) * classes;
+    const Vectors<T> w(o, classes);
+    const int u0 = blockIdx.y * part, u1 = u0 + part < w.count ? u0 + part : w.count;
     const int64_t y = on ? labels[row] : ignore;
-    const RowGrad d(stats, u, on ? row : 0, y, ignore, classes, k);
+    // the given terms, one lane each (k < LANES): the alternatives', behind them the label's, which an
+    // alternative of the same class takes along
+    const int g = (int)(threadIdx.x & 63) % LANES;
+    const bool top = u.top && on && g < k;
+    const int64_t pj = top ? top_idx[row * k + g] : g == k && u.lp && y != ignore ? y : -1;
+    const bool given = pj >= 0 && pj < classes;
+    const float pz = given ? T::one(z + pj) : 0.f;
+    float more = top ? u.top[row * k + g] : 0.f;
+    const RowGrad d(stats, u, on ? row : 0, y, ignore, classes, u.top ? sum_of<LANES>(more) : 0.f);
     const bool plain = !d.r.far && !d.r.bad() && !d.r.dead();
     if (on) {
-        for (int64_t j = first + lane * V; j < end; j += LANES * V) {
-            if (j + V <= end && plain) {
-                float v[V];
-                T::unpack(load16<T>(z + j), v);
+        for (int v0 = u0 + lane; v0 < u1; v0 += LANES * B) {
+            uint4 q[B];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float x = fmaxf(fmaf(v[i], kL, -d.r.ml) - d.r.ls, kFloor);
-                    v[i] = -__builtin_amdgcn_exp2f(x) * fmaf(d.gh, x + d.h, d.g);
+            for (int c = 0; c < B; ++c) {
+                int v = v0 + c * LANES;
+                v = v < w.lo ? w.lo : v > w.hi ? w.hi : v;
+                q[c] = load16<T>(z + w.first_class(v));
+            }
+#pragma unroll
+            for (int c = 0; c < B; ++c) {
+                const int v = v0 + c * LANES, j = w.first_class(v);
+                if (v >= u1) break;
+                if (w.whole(v) && plain) {
+                    float f[V];
+                    T::unpack(q[c], f);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float x = fmaxf(fmaf(f[i], kL, -d.r.ml) - d.r.ls, kFloor);
+                        f[i] = -__builtin_amdgcn_exp2f(x) * fmaf(d.gh, x + d.h, d.g);
+                    }
+                    *(uint4*)(o + j) = T::pack(f);
+                } else {
+                    for (int i = j < 0 ? 0 : j; i < j + V && i < classes; ++i) T::put(o + i, d.value(T::one(z + i)));
                 }
-                store16<T>(o + j, T::pack(v));
-            } else {
-                for (int64_t i = j; i < j + V && i < end; ++i) T::put(o + i, d.value(T::one(z + i)));
             }
         }
     }
     if (!u.top && !u.lp) return;
+    const bool same = top && pj == y;
+    uint64_t any = __ballot(same);
+    if (LANES == 16) any = any >> (threadIdx.x & 48) & 0xFFFF;
+    if (same || g == k) more += d.lp;
     __syncthreads();   // behind the stores of the others
-    if (!on || d.r.dead()) return;
-    // the given terms: the label's and the alternatives', the first of equal classes takes them all
-    for (int i = lane; i <= k; i += LANES) {
-        const int64_t j = i < k ? (u.top ? top_idx[row * k + i] : -1) : y == ignore ? -1 : y;
-        if (j < first || j >= end) continue;
-        if (i == k && u.top) {
-            bool taken = false;
-            for (int e = 0; e < k; ++e) taken |= top_idx[row * k + e] == j;
-            if (taken) continue;
-        }
-        float more = i < k ? u.top[row * k + i] : d.lp;
-        if (i < k && y == j) more += d.lp;
-        T::put(o + j, d.value(T::one(z + j)) + more);
-    }
+    if (LANES > 64 && threadIdx.x >= 64) return;
+    const int u_of = (int)((pj + w.skip) / V);
+    if (given && !(g == k && any) && u_of >= u0 && u_of < u1 && !d.r.dead()) T::put(o + pj, d.value(pz) + more);
 }
 
 template <class T, int ROWS>
@@ -1003,9 +1020,20 @@ k_label_bwd_small(const typename T::type* __restrict__ logits, int64_t n, int cl
     const int pitch = classes | 1;
     if ((int)threadIdx.x < rows) {
         const int64_t row = row0 + threadIdx.x, y = labels[row];
-        const RowGrad d(stats, u, row, y, ignore, classes, k);
+        float top = 0.f;
+        if (u.top)
+            for (int i = 0; i < k; ++i) top += u.top[row * k + i];
+        const RowGrad d(stats, u, row, y, ignore, classes, top);
         float* z = s_z + threadIdx.x * pitch;
-        for (int j = 0; j < classes; ++j) z[j] = d.value(z[j]);
+        if (!d.r.far && !d.r.bad() && !d.r.dead()) {
+#pragma unroll 4
+            for (int j = 0; j < classes; ++j) {
+                const float x = fmaxf(fmaf(z[j], kL, -d.r.ml) - d.r.ls, kFloor);
+                z[j] = -__builtin_amdgcn_exp2f(x) * fmaf(d.gh, x + d.h, d.g);
+            }
+        } else {
+            for (int j = 0; j < classes; ++j) z[j] = d.value(z[j]);
+        }
         if (!d.r.dead()) {
             if (y != ignore && y >= 0 && y < classes) z[y] += d.lp;
             if (u.top && !d.r.bad())
@@ -1013,9 +1041,18 @@ k_label_bwd_small(const typename T::type* __restrict__ logits, int64_t n, int cl
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * classes; e += ROWS) {
-        T::put(out + row0 * classes + e, s_z[e + (int)(__umul24((uint32_t)e, magic) >> 20) * (pitch - classes)]);
+    constexpr int V = T::N;
+    const int all = rows * classes, pad = pitch - classes;
+    const auto at = [&](int e) { return e + (int)(__umul24((uint32_t)e, magic) >> 20) * pad; };
+    typename T::type* o = out + row0 * classes;
+    const int vecs = ((uintptr_t)o & 15) == 0 ? all / V : 0;
+    for (int v = threadIdx.x; v < vecs; v += ROWS) {
+        float f[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = s_z[at(v * V + i)];
+        *(uint4*)(o + v * V) = T::pack(f);
     }
+    for (int e = vecs * V + threadIdx.x; e < all; e += ROWS) T::put(o + e, s_z[at(e)]);
 }
 
 // ---- host
@@ -1159,23 +1196,21 @@ int run_backward(const Call& a, const int64_t* top_idx, const float* stats, cons
                                u, o);
         return launch_status();
     }
-    const int lanes = a.classes <= 16 * T::N * 4 ? 16 : a.classes <= 64 * T::N * 8 ? 64 : 256;
-    int64_t part = a.classes, parts = 1;
-    if (lanes == 256) {
-        part = 256 * T::N * 4;
-        parts = (a.classes + part - 1) / part;
-    }
+    const int lanes = a.classes <= 16 * T::N * 4 && a.k < 16 ? 16 : a.classes <= 64 * T::N * 8 ? 64 : 256;
+    const int64_t vecs = (a.classes + 2 * T::N - 2) / T::N;
+    const int part = lanes == 256 ? 256 * 4 : (int)vecs;
+    const int64_t parts = (vecs + part - 1) / part;
     const int64_t blocks = (a.n + 256 / lanes - 1) / (256 / lanes);
     if (blocks > 0x7FFFFFFFll || parts > 65535) return PIN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks, (unsigned)parts);
     if (lanes == 16)
-        hipLaunchKernelGGL((k_label_bwd<T, 16>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
+        hipLaunchKernelGGL((k_label_bwd<T, 16>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride, a.labels,
                            a.ignore, a.k, top_idx, stats, u, part, o);
     else if (lanes == 64)
-        hipLaunchKernelGGL((k_label_bwd<T, 64>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
+        hipLaunchKernelGGL((k_label_bwd<T, 64>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride, a.labels,
                            a.ignore, a.k, top_idx, stats, u, part, o);
     else
-        hipLaunchKernelGGL((k_label_bwd<T, 256>), grid, dim3(256), 0, a.st, z, a.n, a.classes, a.row_stride, a.labels,
+        hipLaunchKernelGGL((k_label_bwd<T, 256>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride, a.labels,
                            a.ignore, a.k, top_idx, stats, u, part, o);
     return launch_status();
 }
