@@ -46,6 +46,7 @@ struct F32 {
         return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
     static __device__ __forceinline__ float one(const float* p) { return *p; }
+    static __device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 };
 
@@ -67,6 +68,7 @@ struct F16 {
         return __builtin_bit_cast(uint4, h);
     }
     static __device__ __forceinline__ float one(const _Float16* p) { return (float)*p; }
+    static __device__ __forceinline__ uint32_t bits(const _Float16* p) { return *(const uint16_t*)p; }
     static __device__ __forceinline__ void put(_Float16* p, float v) { *p = (_Float16)v; }
 };
 
@@ -91,6 +93,7 @@ struct BF16 {
         return __builtin_bit_cast(uint4, h);
     }
     static __device__ __forceinline__ float one(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+    static __device__ __forceinline__ uint32_t bits(const uint16_t* p) { return *p; }
     static __device__ __forceinline__ void put(uint16_t* p, float v) {
         *p = __builtin_bit_cast(uint16_t, (__bf16)v);
     }
@@ -107,23 +110,18 @@ template <class T>
 __device__ __forceinline__ void store16(typename T::type* p, const uint4& q) {
     __builtin_memcpy(p, &q, 16);
 }
-// the elements [from, to) of sixteen bytes, the others -inf
+// the elements [from, to) of sixteen bytes, from < to, the others -inf (all reads on their way at once: in
+// the others' places the nearest element is read)
 template <class T>
 __device__ __forceinline__ uint4 load_some(const typename T::type* p, int from, int to) {
-    uint32_t u[4] = {T::kFill, T::kFill, T::kFill, T::kFill};
-    if (sizeof(typename T::type) == 4) {
+    uint32_t u[4] = {0, 0, 0, 0};
+    constexpr int V = T::N, W = V / 4;   // elements, elements of 32 bits
+    uint32_t e[V];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i >= from && i < to) __builtin_memcpy(&u[i], (const char*)p + 4 * i, 4);
-    } else {
+    for (int i = 0; i < V; ++i) e[i] = T::bits(p + (i < from ? from : i < to ? i : to - 1));
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i >= from && i < to) {
-                uint16_t h;
-                __builtin_memcpy(&h, (const char*)p + 2 * i, 2);
-                u[i / 2] = i & 1 ? (u[i / 2] & 0xFFFFu) | (uint32_t)h << 16 : (u[i / 2] & 0xFFFF0000u) | h;
-            }
-    }
+    for (int i = 0; i < V; ++i)
+        u[i / W] |= (i < from || i >= to ? T::kFill & (0xFFFFFFFFu >> (32 - 32 / W)) : e[i]) << (i % W * 16);
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
@@ -202,6 +200,9 @@ struct AddF {
     __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
     }
+};
+struct MinU {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
 };
 struct MaxU {
     __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
@@ -505,6 +506,102 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
     if (gt > 256) return largest_by_passes<T, 64>(zr, classes, k, s_c.gt, emit);
     if (eq > 256) eq = first_equal<T, 64>(zr, 0, classes, kth, k - gt, 0, s_c.eq, s_tot);
     s_c.sort(gt, eq, k, emit);
+}
+
+// Sixteen lanes per row, 16 NCH vectors: four rows share what a wave spends on reductions.  Alternatives, few
+// of them: the row's largest, then the first class that has it (looked for in the vectors whose maximum it is),
+// which is marked and its vector's maximum taken again.
+template <class T, int NCH, bool TOP>
+__global__ void __launch_bounds__(256)
+k_label_lanes(const typename T::type* __restrict__ logits, int64_t n, int classes, int64_t row_stride,
+              const int64_t* __restrict__ labels, int64_t ignore, int k, Out out) {
+    constexpr int V = T::N;
+    const int lane = threadIdx.x & 15;
+    const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), row = at < n ? at : n - 1;
+    const bool writes = at < n && lane == 0;
+    const typename T::type* zr = logits + row * row_stride;
+    const Vectors<T> z(zr, classes);
+    const int most = (classes + 2 * V - 2) / V;   // vectors of a row at any alignment
+    uint4 q[NCH];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) q[c] = z.load_near(c * 16 + lane);
+    const int64_t y = labels[row];
+    const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
+    float cm[NCH], mx = -kInf;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const int u = c * 16 + lane;
+        if (!z.whole(u)) q[c] = z.load_edge(u);
+        cm[c] = vector_max<T>(q[c]);
+        mx = max_nan(mx, cm[c]);
+    }
+    mx = mx != mx ? kInf : mx;
+    Row r(__uint_as_float(rows_of_16(__float_as_uint(mx), MaxF())));
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) forget(q[c]);
+    float s = 0.f, t = 0.f;
+    const float off = r.far ? 0.f : r.ml, from = r.far ? r.m : 0.f;   // x = (z - from) L - off
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        if (c > 0 && c * 16 >= most) break;   // the same for all threads
+        float v[V];
+        T::unpack(q[c], v);
+        if (__any(r.far)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] -= from;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float x = fmaxf(fmaf(v[i], kL, -off), kFloor), e = __builtin_amdgcn_exp2f(x);
+            s += e;
+            t = fmaf(e, x, t);
+        }
+    }
+    s = __uint_as_float(rows_of_16(__float_as_uint(s), AddF()));
+    t = __uint_as_float(rows_of_16(__float_as_uint(t), AddF()));
+    r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
+    if (writes) put_row(out, r, row, s, t, zy, y, ignore, classes);
+    if (!TOP) return;
+    uint64_t taken = 0;   // a bit per element (V NCH <= 64)
+    const auto is_taken = [&](int c, int i) { return (taken >> (c * V + i) & 1) != 0; };
+    for (int e = 0; e < k; ++e) {
+        float best = cm[0];
+#pragma unroll
+        for (int c = 1; c < NCH; ++c) best = fmaxf(best, cm[c]);
+        best = __uint_as_float(rows_of_16(__float_as_uint(best), MaxF()));
+        int j = classes;   // my first class that has it
+#pragma unroll
+        for (int c = NCH - 1; c >= 0; --c) {
+            if (cm[c] == best) {
+                float v[V];
+                T::unpack(q[c], v);
+                const int j0 = z.first_class(c * 16 + lane);
+#pragma unroll
+                for (int i = V - 1; i >= 0; --i)
+                    j = v[i] == best && !is_taken(c, i) && (unsigned)(j0 + i) < (unsigned)classes ? j0 + i : j;
+            }
+        }
+        const int first = (int)rows_of_16((uint32_t)j, MinU());
+        if (writes) {
+            out.top_lp[row * k + e] = r.log_prob(best);
+            out.top_idx[row * k + e] = r.bad() ? -1 : first;
+        }
+        if (e + 1 < k && j == first && j < classes) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int i0 = first - z.first_class(c * 16 + lane);
+                if ((unsigned)i0 < (unsigned)V) {
+                    taken |= 1ull << (c * V + i0);
+                    float v[V];
+                    T::unpack(q[c], v);
+                    float m = -kInf;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) m = fmaxf(m, is_taken(c, i) ? -kInf : v[i]);
+                    cm[c] = m;
+                }
+            }
+        }
+    }
 }
 
 // A part of a long row: its maximum and sums, and for the alternatives the maxima of 64 groups of its
@@ -1070,14 +1167,29 @@ struct Plan {
     int nch;       // one wave per row, nch vectors per lane; 0: parts of `part` vectors, `splits` of them
     int splits, part;
     int alone;     // a workgroup goes through a row alone, this many parts
+    int lanes;     // sixteen lanes per row, this many vectors each
 };
 
+// Sixteen lanes per row look at their elements once per alternative, a wave per row at a few more than k in
+// all, after a longer preparation.  200000 x 128 bf16 with 3 alternatives: 47 us and 121; 16384 x 1003 f16
+// with 8: 50 and 24.  A wave whose lanes with elements are hardly more than k finds no bound by them: 200000 x
+// 128 with 20: 191 and 485.  With few rows it is the longest row that counts: 64 x 1003 with 8: 23 us and 6.
+constexpr int64_t kManyRows = 4096;
 constexpr int64_t kFull = 1024;    // workgroups that fill the chip
 constexpr int64_t kRows = 256;     // rows that do when each has a workgroup
 
-Plan plan_rows(int64_t n, int64_t classes, int v) {
+Plan plan_rows(int64_t n, int64_t classes, int v, int k) {
     const int64_t vecs = (classes + 2 * v - 2) / v;   // at any alignment
-    Plan p{1, 1, (int)vecs, 0};
+    Plan p{1, 1, (int)vecs, 0, 0};
+    if (vecs <= 16 * 8) {
+        int nch = 1;
+        while (16 * nch < vecs) nch *= 2;
+        const int looks = k * nch * v;   // elements a lane looks at for all alternatives
+        if (looks <= (n < kManyRows ? 32 : 160) || (vecs <= 2 * k && n >= kManyRows)) {
+            p.lanes = nch;
+            return p;
+        }
+    }
     if (vecs <= 64 * 8) {
         while (64 * p.nch < vecs) p.nch *= 2;
         return p;
@@ -1124,6 +1236,18 @@ void launch_wave(const Call& a) {
                            a.row_stride, a.labels, a.ignore, a.k, a.out);
 }
 
+template <class T, int NCH>
+void launch_lanes(const Call& a) {
+    const typename T::type* z = (const typename T::type*)a.logits;
+    const dim3 grid((unsigned)((a.n + 15) / 16));
+    if (a.k > 0)
+        hipLaunchKernelGGL((k_label_lanes<T, NCH, true>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride,
+                           a.labels, a.ignore, a.k, a.out);
+    else
+        hipLaunchKernelGGL((k_label_lanes<T, NCH, false>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride,
+                           a.labels, a.ignore, a.k, a.out);
+}
+
 template <class T>
 int run_forward(const Call& a) {
     if (a.classes <= kSmall) {
@@ -1142,8 +1266,15 @@ int run_forward(const Call& a) {
         else go(k_label_small<T, 128, 64>);
         return launch_status();
     }
-    const Plan p = plan_rows(a.n, a.classes, T::N);
+    const Plan p = plan_rows(a.n, a.classes, T::N, a.k);
     if (a.n * p.splits > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
+    if (p.lanes > 0) {
+        if (p.lanes == 1) launch_lanes<T, 1>(a);
+        else if (p.lanes == 2) launch_lanes<T, 2>(a);
+        else if (p.lanes == 4) launch_lanes<T, 4>(a);
+        else launch_lanes<T, 8>(a);
+        return launch_status();
+    }
     if (p.nch > 0) {
         if (p.nch == 1) launch_wave<T, 1>(a);
         else if (p.nch == 2) launch_wave<T, 2>(a);
@@ -1224,8 +1355,8 @@ int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dt
         top_k < 0 || top_k > PIN_LABEL_TOP_MAX)
         return PIN_ERR_ARG;
     if (n == 0 || classes <= kSmall) return 0;
-    const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N);
-    return p.nch > 0 || p.alone > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
+    const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N, top_k);
+    return p.lanes > 0 || p.nch > 0 || p.alone > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
 }
 
 int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,

@@ -350,9 +350,8 @@ def test_places_past_32_bits(dev):
     z = buf.as_strided((2, c), (far, 1))
     logits, y = make(2, c, torch.bfloat16, dev)
     z.copy_(logits)
-    got = P.label_log_probs(z, y, top_k=5)
-    want = P.label_log_probs(logits, y, top_k=5)
-    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # (a row's vectors begin where its address does, so the sums' order, and their last bits, go by the place)
+    check(z, y, 5, grads=False)
 
 
 def test_gradient_past_32_bits(dev):
