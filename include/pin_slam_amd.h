@@ -945,7 +945,7 @@ int pin_mc_emit(const float* values, int64_t nx, int64_t ny, int64_t nz, float l
 #define PIN_TYPE_BF16 2
 
 #define PIN_LABEL_TOP_MAX 32             /* most alternatives per row */
-#define PIN_LABEL_CLASSES_MAX 2097152    /* most classes (2^21) */
+#define PIN_LABEL_CLASSES_MAX 524280     /* most classes */
 
 /*
  * pin_label_logprob -- for each of n rows of `classes` logits (type `dtype`, consecutive classes

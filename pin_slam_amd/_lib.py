@@ -121,7 +121,7 @@ class PinRowArray(ctypes.Structure):
 ROW_ARRAYS_MAX = 8   # PIN_ROW_ARRAYS_MAX
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # PIN_TYPE_*
 LABEL_TOP_MAX = 32             # PIN_LABEL_TOP_MAX
-LABEL_CLASSES_MAX = 1 << 21    # PIN_LABEL_CLASSES_MAX
+LABEL_CLASSES_MAX = 524280     # PIN_LABEL_CLASSES_MAX
 ADAMW_BLOCK = 256              # PIN_ADAMW_BLOCK
 ADAMW_SCALARS_BYTES = 64       # PIN_ADAMW_SCALARS_BYTES
 MLP_GRAD_FIRST, MLP_GRAD_SECOND = 1, 2   # pin_mlp_backward flags

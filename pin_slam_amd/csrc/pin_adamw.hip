@@ -31,6 +31,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kGroup = PIN_ADAMW_BLOCK;       // elements that share their exponents
 constexpr int kChunk = 1024;                  // elements of one workgroup
+constexpr int64_t kChunks = 0xFFFFFFFFll / kBlock;   // workgroups of one launch: it has fewer than 2^32 threads
 constexpr int kTensors = 112;                 // tensors of one launch (its table is a kernel argument)
 static_assert(kTensors <= 128, "the table is searched by two ballots");
 constexpr uint32_t kMix1 = 0x9E3779B1u, kMix2 = 0x6A09E667u, kMix3 = 0xBB67AE85u;   // fractional bits of the
@@ -364,8 +365,8 @@ int pin_adamw_step(void* const* params, const void* const* grads, const int64_t*
     int64_t chunks = 0;
     for (int32_t k = 0; k <= count; ++k) {
         const int64_t more = k < count ? (sizes[k] + kChunk - 1) / kChunk : 0;
-        if (more > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
-        if (t.count > 0 && (k == count || t.count == kTensors || chunks + more > 0x7FFFFFFFll)) {
+        if (more > kChunks) return PIN_ERR_UNSUPPORTED;
+        if (t.count > 0 && (k == count || t.count == kTensors || chunks + more > kChunks)) {
             if (dtype == PIN_TYPE_F32)
                 launch_adamw<float>(t, (uint32_t)chunks, state_bits, exp_avg, exp_avg_sq, exponents, master, (float)eps, a,
                                     (const AdamwScalars*)scalars, as_stream(stream));
@@ -400,7 +401,7 @@ int pin_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const int16_t
     if (((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)exponents) & 3 || ((uintptr_t)m | (uintptr_t)v) & 15)
         return PIN_ERR_ARG;
     const int64_t blocks = (n / 4 + kBlock - 1) / kBlock;
-    if (blocks > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
+    if (blocks > kChunks) return PIN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(k_adamw_moments, dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
                        (const uint32_t*)exp_avg, (const uint32_t*)exp_avg_sq, (const short2*)exponents, n / 4, (float4*)m,
                        (float4*)v);

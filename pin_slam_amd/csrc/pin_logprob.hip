@@ -803,6 +803,7 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
 // maximum of its own (2^x is taken to it, and what it has summed is taken to a new one), so nothing waits
 // for the other threads before the row's end.
 constexpr int kPart = 256 * 4;     // vectors of a part
+static_assert((PIN_LABEL_CLASSES_MAX + 6) / 4 <= (int64_t)kSplits * 2 * kPart, "the longest row's parts");
 constexpr int kRowParts = 32;      // most parts of a row here (their groups' maxima lie in LDS)
 
 template <class T>
@@ -1176,7 +1177,11 @@ struct Plan {
 // 128 with 20: 191 and 485.  With few rows it is the longest row that counts: 64 x 1003 with 8: 23 us and 6.
 constexpr int64_t kManyRows = 4096;
 constexpr int64_t kFull = 1024;    // workgroups that fill the chip
-constexpr int64_t kRows = 256;     // rows that do when each has a workgroup
+constexpr int64_t kBatch = 1 << 23;  // rows of one launch
+// ... when each has a workgroup to itself, or its rows are short: 256 x 50021 bf16 with 20 alternatives 16.8 us
+// (in parts, joined, 21.9), 1 x 32768 with 5 8.0 (9.0), but 1 x 131072 with 20 19.6 (12.5).
+constexpr int64_t kRows = 256;
+constexpr int64_t kShort = 6;
 
 Plan plan_rows(int64_t n, int64_t classes, int v, int k) {
     const int64_t vecs = (classes + 2 * v - 2) / v;   // at any alignment
@@ -1196,7 +1201,7 @@ Plan plan_rows(int64_t n, int64_t classes, int v, int k) {
     }
     p.nch = 0;
     const int64_t parts = (vecs + kPart - 1) / kPart;
-    if (parts <= kRowParts && (n >= kRows || parts <= 2)) {
+    if (parts <= kRowParts && (n >= kRows || parts <= kShort)) {
         p.part = kPart;
         p.alone = (int)parts;
         return p;
@@ -1249,11 +1254,10 @@ void launch_lanes(const Call& a) {
 }
 
 template <class T>
-int run_forward(const Call& a) {
+int forward_rows(const Call& a, const Plan& p) {
     if (a.classes <= kSmall) {
         const int rows = a.classes <= 32 ? 256 : 128;
         const int64_t blocks = (a.n + rows - 1) / rows;
-        if (blocks > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
         const size_t lds = (size_t)rows * (a.classes | 1) * 4;
         const typename T::type* z = (const typename T::type*)a.logits;
         const auto go = [&](auto kernel) {
@@ -1266,8 +1270,7 @@ int run_forward(const Call& a) {
         else go(k_label_small<T, 128, 64>);
         return launch_status();
     }
-    const Plan p = plan_rows(a.n, a.classes, T::N, a.k);
-    if (a.n * p.splits > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
+    if (a.n * p.splits > kBatch * 2) return PIN_ERR_UNSUPPORTED;   // (n of a batch, or n < kFull and few parts)
     if (p.lanes > 0) {
         if (p.lanes == 1) launch_lanes<T, 1>(a);
         else if (p.lanes == 2) launch_lanes<T, 2>(a);
@@ -1308,14 +1311,32 @@ int run_forward(const Call& a) {
     return launch_status();
 }
 
+// Rows in batches: a launch has fewer than 2^32 threads.
 template <class T>
-int run_backward(const Call& a, const int64_t* top_idx, const float* stats, const Grads& u, void* d_logits) {
+int run_forward(const Call& a) {
+    const Plan p = plan_rows(a.n, a.classes, T::N, a.k);
+    for (int64_t row = 0; row < a.n; row += kBatch) {
+        Call b = a;
+        b.n = a.n - row < kBatch ? a.n - row : kBatch;
+        b.logits = (const typename T::type*)a.logits + row * a.row_stride;
+        b.labels += row;
+        b.out.log_prob += row;
+        b.out.entropy += row;
+        if (a.out.stats) b.out.stats += 3 * row;
+        if (a.k > 0) b.out.top_lp += row * a.k, b.out.top_idx += row * a.k;
+        const int rc = forward_rows<T>(b, p);
+        if (rc != PIN_OK) return rc;
+    }
+    return PIN_OK;
+}
+
+template <class T>
+int backward_rows(const Call& a, const int64_t* top_idx, const float* stats, const Grads& u, void* d_logits) {
     typename T::type* o = (typename T::type*)d_logits;
     const typename T::type* z = (const typename T::type*)a.logits;
     if (a.classes <= kSmall) {
         const int rows = a.classes <= 32 ? 256 : 128;
         const int64_t blocks = (a.n + rows - 1) / rows;
-        if (blocks > 0x7FFFFFFFll) return PIN_ERR_UNSUPPORTED;
         const size_t lds = (size_t)rows * (a.classes | 1) * 4;
         if (rows == 256)
             hipLaunchKernelGGL((k_label_bwd_small<T, 256>), dim3((unsigned)blocks), dim3(256), lds, a.st, z, a.n,
@@ -1332,7 +1353,7 @@ int run_backward(const Call& a, const int64_t* top_idx, const float* stats, cons
     const int part = lanes == 256 ? 256 * 4 : (int)vecs;
     const int64_t parts = (vecs + part - 1) / part;
     const int64_t blocks = (a.n + 256 / lanes - 1) / (256 / lanes);
-    if (blocks > 0x7FFFFFFFll || parts > 65535) return PIN_ERR_UNSUPPORTED;
+    if (parts > 65535) return PIN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks, (unsigned)parts);
     if (lanes == 16)
         hipLaunchKernelGGL((k_label_bwd<T, 16>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride, a.labels,
@@ -1344,6 +1365,21 @@ int run_backward(const Call& a, const int64_t* top_idx, const float* stats, cons
         hipLaunchKernelGGL((k_label_bwd<T, 256>), grid, dim3(256), 0, a.st, z, a.n, (int)a.classes, a.row_stride, a.labels,
                            a.ignore, a.k, top_idx, stats, u, part, o);
     return launch_status();
+}
+
+template <class T>
+int run_backward(const Call& a, const int64_t* top_idx, const float* stats, const Grads& u, void* d_logits) {
+    for (int64_t row = 0; row < a.n; row += kBatch) {
+        Call b = a;
+        b.n = a.n - row < kBatch ? a.n - row : kBatch;
+        b.logits = (const typename T::type*)a.logits + row * a.row_stride;
+        b.labels += row;
+        const Grads v{u.lp ? u.lp + row : nullptr, u.ent ? u.ent + row : nullptr, u.top ? u.top + row * a.k : nullptr};
+        const int rc = backward_rows<T>(b, top_idx ? top_idx + row * a.k : nullptr, stats + 3 * row, v,
+                                        (typename T::type*)d_logits + row * a.classes);
+        if (rc != PIN_OK) return rc;
+    }
+    return PIN_OK;
 }
 
 }  // namespace

@@ -102,11 +102,17 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "capturable": self.capturable, "seed": self.seed, "_arenas": self._arenas}
+
+    def _check_lr(self, lr, device):
+        if not self.capturable or lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device:
+            raise ValueError("AdamW: a tensor lr must be one float32 on the parameters' device, with capturable=True")
+
     def _check_group(self, group):
         lr, (b1, b2) = group["lr"], group["betas"]
         if isinstance(lr, torch.Tensor):
-            if not self.capturable or lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
-                raise ValueError("AdamW: a tensor lr must be one float32 on the device, with capturable=True")
+            self._check_lr(lr, group["params"][0].device)
         elif not 0.0 <= lr < float("inf"):
             raise ValueError(f"AdamW: lr must be >= 0 (got {lr})")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
@@ -205,6 +211,8 @@ class AdamW(torch.optim.Optimizer):
             if not self.capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: capturing a step needs capturable=True (the step count is on the host)")
             arena = self._arena(gi)
+            if isinstance(group["lr"], torch.Tensor):
+                self._check_lr(group["lr"], arena.device)
             work.append((gi, group, arena, self._gather(arena, group)))
         for gi, group, arena, todo in work:
             with _lib.on_device(arena.device):
@@ -218,7 +226,7 @@ class AdamW(torch.optim.Optimizer):
         lr, (b1, b2) = group["lr"], group["betas"]
         stream = _lib.stream(arena.device)
         wd, salt = float(group["weight_decay"]), self._salt(gi)
-        lr_dev = lr if isinstance(lr, torch.Tensor) else None
+        lr_dev = lr if isinstance(lr, torch.Tensor) and self.capturable else None
         rates = (0.0 if lr_dev is not None else float(lr), float(b1), float(b2))
         if self.capturable:
             _lib.call("pin_adamw_scalars", _lib.ptr(arena.step_dev), _lib.ptr(lr_dev), *rates, wd, salt,
@@ -314,11 +322,19 @@ class AdamW(torch.optim.Optimizer):
         for mine, saved in zip(self.param_groups, groups):
             mine.update({key: val for key, val in saved.items() if key != "params"})
             self._check_group(mine)
+        to, by = {}, {}
         for gi, i, p, want, one in plan:
             arena = self._arena(gi)
             for key in want:
-                self.state[p][key].copy_(one[key])
+                pair = to.setdefault((gi, one[key].dtype, one[key].device), ([], []))
+                pair[0].append(self.state[p][key])
+                pair[1].append(one[key])
             arena.steps[i] = int(one["step"])
-            arena.together = len(set(arena.steps)) == 1
             if arena.step_dev is not None:
-                arena.step_dev.fill_(arena.steps[i])
+                by[gi] = arena.steps[i]
+        for mine, saved in to.values():
+            torch._foreach_copy_(mine, saved)
+        for arena in self._arenas.values():
+            arena.together = len(set(arena.steps)) == 1
+        for gi, step in by.items():
+            self._arenas[gi].step_dev.fill_(step)

@@ -76,7 +76,7 @@ def test_argument_errors_before_any_device_work():
         return lib.pin_label_logprob(logits, dtype, n, c, stride, labels, -100, k, lp, ent, None, top, idx, None, None)
 
     assert logprob(n=0) == 0
-    for bad in (dict(logits=None), dict(dtype=3), dict(dtype=-1), dict(n=-1), dict(c=0), dict(c=(1 << 21) + 1),
+    for bad in (dict(logits=None), dict(dtype=3), dict(dtype=-1), dict(n=-1), dict(c=0), dict(c=524281),
                 dict(stride=-1), dict(labels=None), dict(k=11), dict(k=33, c=100), dict(k=-1), dict(lp=None),
                 dict(ent=None), dict(top=None), dict(idx=None), dict(logits=ctypes.c_void_p(4098))):
         assert logprob(**bad) == -1, bad

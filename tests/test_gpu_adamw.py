@@ -390,6 +390,36 @@ def test_captured_and_replayed(dev, bits):
     assert opt.state_dict()["state"][0]["step"] == 5
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copied_with_its_parameters(dev, bits):
+    a = tensors([1000, 33], torch.float32, dev)
+    opt = P.AdamW(a, state_bits=bits, seed=5, **HYPER)
+    set_grads(a, 1)
+    opt.step()
+    b, other = copy.deepcopy((a, opt))
+    for t in (2, 3):
+        for params, o in ((a, opt), (b, other)):
+            set_grads(params, t)
+            o.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and p.data_ptr() != q.data_ptr()
+
+
+def test_a_tensor_lr_is_checked_at_each_step(dev):
+    p = tensors([100], torch.float32, dev)
+    set_grads(p, 1)
+    plain = P.AdamW(p, **HYPER)
+    plain.param_groups[0]["lr"] = torch.tensor([0.1], device=dev)
+    with pytest.raises(ValueError, match="tensor lr"):
+        plain.step()
+    opt = P.AdamW(p, capturable=True, **{**HYPER, "lr": torch.tensor([0.1], device=dev)})
+    opt.step()
+    for bad in (torch.tensor([0.1]), torch.tensor([0.1], device=dev, dtype=torch.float64), torch.zeros(2, device=dev)):
+        opt.param_groups[0]["lr"] = bad
+        with pytest.raises(ValueError, match="tensor lr"):
+            opt.step()
+
+
 def test_capture_refusals(dev):
     p = tensors([100], torch.float32, dev)
     set_grads(p, 1)

@@ -157,7 +157,8 @@ def make(n, c, kind, dev, pad=0, seed=0, ignore_some=True):
 
 SIZES = [(1, 1), (1, 2), (2, 3), (300, 20), (1025, 19), (9, 31), (70, 32), (5, 33), (7, 63), (130, 64), (4, 65), (3, 127),
          (11, 255), (6, 257), (513, 500), (3, 1003), (2, 2047), (5, 4097), (3, 8191), (2, 8192), (3, 16385), (2, 32769),
-         (1, 50021), (3, 65537), (1, 131072), (2, 140001)]
+         (1, 50021), (3, 65537), (1, 131072), (2, 140001), (2, 300001), (1, 524280), (5000, 70), (4099, 130), (4100, 301),
+         (4096, 1000), (260, 20003)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
@@ -256,14 +257,38 @@ def test_masks_ties_and_values(dev, c, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-def test_large_values_in_one_place(dev, kind):
+@pytest.mark.parametrize("c,times", [(100, 171), (700, 171), (20003, 11)])
+def test_masks_ties_and_values_of_many_rows(dev, c, times, kind):
+    """The same rows where so many are laid out otherwise on the chip."""
+    z, y = special_rows(c, TYPES[kind])
+    for k in (0, 2, 5, 32):
+        check(z.repeat(times, 1).to(dev), y.repeat(times).to(dev), k)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("times", [1, 33])
+def test_large_values_in_one_place(dev, kind, times):
     """All of the largest values next to one another (one lane's, one wave's, one workgroup's): the alternatives
     come from one place, in order."""
     c = 70001
     z = torch.randn((8, c), generator=torch.Generator().manual_seed(7))
     for r, a in enumerate([0, 8, 64, 500, 4096, 16000, 32768, c - 3000]):
         z[r, a:a + 3000] = torch.linspace(50.0, 20.0, 3000) if r % 2 else torch.linspace(20.0, 50.0, 3000)
-    check(z.to(TYPES[kind]).to(dev), torch.arange(8, device=dev) * 5000, 32)
+    check(z.repeat(times, 1).to(TYPES[kind]).to(dev), (torch.arange(8, device=dev) * 5000).repeat(times), 32, grads=times == 1)
+
+
+def test_more_rows_than_one_launch_takes(dev):
+    """2^23 + 3 rows (one row's memory): the last rows' values and gradients are the first's."""
+    n, c = (1 << 23) + 3, 300
+    row, y = make(1, c, torch.bfloat16, dev, ignore_some=False)
+    got = P.label_log_probs(row.expand(n, c), y.expand(n), top_k=8)
+    for t in got:
+        assert torch.equal(t[-5:], t[:1].expand(5, *t.shape[1:]))
+    check(row.expand(4097, c), y.expand(4097), 8)
+    x = row[:, :5].expand(n, 5).requires_grad_(True)
+    r = P.label_log_probs(x, y.expand(n) % 5, top_k=2)
+    dz, = torch.autograd.grad([r.log_prob, r.top_log_prob], x, [torch.ones_like(r.log_prob), torch.ones_like(r.top_log_prob)])
+    assert torch.equal(dz[-5:], dz[:1].expand(5, 5)) and bool(dz.any())
 
 
 def test_partial_gradients(dev):
@@ -356,7 +381,7 @@ def test_places_past_32_bits(dev):
 
 def test_gradient_past_32_bits(dev):
     """A gradient of more than 2^31 elements: the last rows are the same as alone."""
-    n, c = 2200, 1000003
+    n, c = 4400, 500003
     z = torch.zeros((1, c), dtype=torch.bfloat16, device=dev)
     z[0, :1000] = torch.randn((1000,), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
     x = z.expand(n, c).requires_grad_(True)
