@@ -291,6 +291,26 @@ def test_more_rows_than_one_launch_takes(dev):
     assert torch.equal(dz[-5:], dz[:1].expand(5, 5)) and bool(dz.any())
 
 
+def test_gradient_through_other_layouts(dev):
+    """Logits that are a transposed, sliced or expanded leaf: the gradient comes back in the leaf's layout."""
+    logits, y = make(6, 40, torch.float32, dev, ignore_some=False)
+    x = logits.detach().clone().requires_grad_(True)
+    want, = torch.autograd.grad(P.label_log_probs(x, y).log_prob.sum(), x)
+    t = logits.t().contiguous().requires_grad_(True)
+    got, = torch.autograd.grad(P.label_log_probs(t.t(), y).log_prob.sum(), t)
+    torch.testing.assert_close(got.t(), want)
+    w = torch.zeros((6, 50), device=dev)
+    w[:, 3:43] = logits
+    w.requires_grad_(True)
+    got, = torch.autograd.grad(P.label_log_probs(w[:, 3:43], y).log_prob.sum(), w)
+    torch.testing.assert_close(got[:, 3:43], want)
+    assert not bool(got[:, :3].any()) and not bool(got[:, 43:].any())
+    one = logits[:1].clone().requires_grad_(True)
+    got, = torch.autograd.grad(P.label_log_probs(one.expand(6, 40), y).log_prob.sum(), one)
+    each = [torch.autograd.grad(P.label_log_probs(one, y[i:i + 1]).log_prob.sum(), one)[0] for i in range(6)]
+    torch.testing.assert_close(got, sum(each))
+
+
 def test_partial_gradients(dev):
     """Each output alone, and expanded upstream gradients."""
     logits, y = make(37, 257, torch.float32, dev)
