@@ -352,62 +352,69 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
     return kth_of_wave<LOW, 1>(one, k);
 }
 
-// What is at or above a bound that is not above the k-th largest: two lists in LDS.
-template <int GT, int EQ>
+// the least value above one (a bound that v reaches if v is larger)
+__device__ __forceinline__ float above(float v) { return key_value(order_key(v) + 1); }
+
+// What reaches a bound that is not above the k-th largest, in LDS; behind it room for equal ones.
+template <int MOST>
 struct Candidates {
-    uint64_t gt[GT], eq[EQ];
-    uint32_t n_gt, n_eq;
-    __device__ __forceinline__ void push(float v, int j, float kth) {
-        if (v > kth) {
-            const uint32_t p = atomicAdd(&n_gt, 1u);
-            if (p < GT) gt[p] = class_key(v, (uint32_t)j);
-        } else if (v == kth) {
-            const uint32_t p = atomicAdd(&n_eq, 1u);
-            if (p < EQ) eq[p] = class_key(v, (uint32_t)j);
+    uint64_t key[MOST + PIN_LABEL_TOP_MAX];
+    uint32_t n;
+    static constexpr int kMost = MOST;
+    // (a lane's hits as bits first: most lanes have one or none, and a turn for each is dearer than a bit)
+    template <class T>
+    __device__ __forceinline__ void push_vector(const Vectors<T>& z, int u, const uint4& q, float bound) {
+        constexpr int V = T::N;
+        float v[V];
+        T::unpack(q, v);
+        const int j = z.first_class(u), lo = j < 0 ? -j : 0, room = z.classes - j, hi = room < 0 ? 0 : room < V ? room : V;
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) hits |= v[i] >= bound ? 1u << i : 0u;
+        hits &= (1u << hi) - (1u << lo);
+        while (__any(hits != 0)) {
+            if (hits != 0) {
+                const int at = __ffs(hits) - 1;
+                float w = v[0];
+#pragma unroll
+                for (int i = 1; i < V; ++i) w = i == at ? v[i] : w;
+                const uint32_t p = atomicAdd(&n, 1u);
+                if (p < MOST) key[p] = class_key(w, (uint32_t)(j + at));
+                hits &= hits - 1;
+            }
         }
     }
-    template <class T>
-    __device__ __forceinline__ void push_vector(const Vectors<T>& z, int u, const uint4& q, float kth) {
-        float v[T::N];
-        T::unpack(q, v);
-        const int j = z.first_class(u);
-#pragma unroll
-        for (int i = 0; i < T::N; ++i)
-            if (v[i] >= kth && j + i >= 0 && j + i < z.classes) push(v[i], j + i, kth);
-    }
-    // one wave: the k largest of the lists' g and e elements, in order; at least k
+    // one wave: the k largest of `all`, in order; at least k
     template <class F>
-    __device__ __forceinline__ void sort(int g, int e, int k, F emit) const {
-        const int lane = threadIdx.x & 63, all = g + e;
+    __device__ __forceinline__ void sort(int all, int k, F emit) const {
+        const int lane = threadIdx.x & 63;
         if (all <= 64) {
-            const uint64_t key = lane < g ? gt[lane] : lane < all ? eq[lane - g] : 0;
+            const uint64_t mine = lane < all ? key[lane] : 0;
             int rank = 0;
             for (int i = 0; i < all; ++i) {
-                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
-                                       (uint32_t)__builtin_amdgcn_readlane((int)key, i);
-                rank += other > key ? 1 : 0;
+                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+                rank += other > mine ? 1 : 0;
             }
-            if (lane < all && rank < k) emit(rank, key);
+            if (lane < all && rank < k) emit(rank, mine);
             return;
         }
         uint64_t last = ~0ull;
         for (int i = 0; i < k; ++i) {
             uint64_t best = 0;
-            for (int p = lane; p < all; p += 64) {
-                const uint64_t key = p < g ? gt[p] : eq[p - g];
-                if (key < last && key > best) best = key;
-            }
+            for (int p = lane; p < all; p += 64)
+                if (key[p] < last && key[p] > best) best = key[p];
             last = wave_max_key(best);
             if (lane == 0) emit(i, last);
         }
     }
 };
 
-// The first `need` classes of [from, to) whose logit is `value`, appended to eq at `have`; all threads
-// of the workgroup (THREADS of them), which may not read eq before.  Returns how many there are now.
+// The first `need` classes of [from, to) whose logit is `value`, put at keys[have] and on; all threads of
+// the workgroup (THREADS of them), behind a barrier.  Returns how many there are now, at most `need`.
 template <class T, int THREADS>
 __device__ __forceinline__ int first_equal(const typename T::type* z, int from, int to, float value, int need, int have,
-                                           uint64_t* eq, uint32_t* s_tot) {
+                                           uint64_t* keys, uint32_t* s_tot) {
     const int wave = threadIdx.x >> 6;
 #pragma unroll 1
     for (int j0 = from; j0 < to && have < need; j0 += THREADS) {
@@ -421,7 +428,7 @@ __device__ __forceinline__ int first_equal(const typename T::type* z, int from, 
             at += w < wave ? (int)s_tot[w] : 0;
             have += (int)s_tot[w];
         }
-        if (v == value && at < need) eq[at] = class_key(v, (uint32_t)j);
+        if (v == value && at < need) keys[at] = class_key(v, (uint32_t)j);
         __syncthreads();
     }
     return have < need ? have : need;
@@ -456,7 +463,7 @@ template <class T, int NCH, bool TOP>
 __global__ void __launch_bounds__(64)
 k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes, int64_t row_stride,
              const int64_t* __restrict__ labels, int64_t ignore, int k, Out out) {
-    __shared__ Candidates<TOP ? 256 : 1, TOP ? 256 : 1> s_c;
+    __shared__ Candidates<TOP ? 256 : 1> s_c;
     __shared__ uint32_t s_tot[1];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
@@ -483,7 +490,7 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);   // s >= 1 unless there is nothing
     if (lane == 0) {
         put_row(out, r, row, s, t, zy, y, ignore, classes);
-        s_c.n_gt = s_c.n_eq = 0;
+        s_c.n = 0;
     }
     if (!TOP) return;
     const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
@@ -495,17 +502,23 @@ k_label_wave(const typename T::type* __restrict__ logits, int64_t n, int classes
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < NCH; ++c) forget(q[c]);
-    if (mx >= kth) {
+    const auto collect = [&](float bound) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
-            if (cm[c] >= kth) s_c.push_vector(z, c * 64 + lane, q[c], kth);
+            if (cm[c] >= bound) s_c.push_vector(z, c * 64 + lane, q[c], bound);
+        __syncthreads();
+        return (int)s_c.n;
+    };
+    int all = collect(kth);
+    if (all > s_c.kMost) {   // many at the bound itself: those above it, and the first of the others
+        __syncthreads();
+        if (lane == 0) s_c.n = 0;
+        __syncthreads();
+        all = collect(above(kth));
+        if (all > s_c.kMost) return largest_by_passes<T, 64>(zr, classes, k, s_c.key, emit);
+        if (all < k) all += first_equal<T, 64>(zr, 0, classes, kth, k - all, 0, s_c.key + all, s_tot);
     }
-    __syncthreads();
-    const int gt = (int)s_c.n_gt;
-    int eq = gt >= k ? 0 : (int)s_c.n_eq;
-    if (gt > 256) return largest_by_passes<T, 64>(zr, classes, k, s_c.gt, emit);
-    if (eq > 256) eq = first_equal<T, 64>(zr, 0, classes, kth, k - gt, 0, s_c.eq, s_tot);
-    s_c.sort(gt, eq, k, emit);
+    s_c.sort(all, k, emit);
 }
 
 // Sixteen lanes per row, 16 NCH vectors: four rows share what a wave spends on reductions.  Alternatives, few
@@ -670,9 +683,7 @@ __device__ __forceinline__ Row join_sums(const float4* __restrict__ sums, const 
     const float f = __builtin_amdgcn_exp2f(x);
     const float s = wave_sum(f * p.y), t = wave_sum(f * fmaf(p.y, x, p.z));
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
-    if (threadIdx.x == 0) {
-        put_row(out, r, row, s, t, zy, y, ignore, classes);
-    }
+    if (threadIdx.x == blockDim.x - 64) put_row(out, r, row, s, t, zy, y, ignore, classes);   // the last wave
     return r;
 }
 
@@ -688,18 +699,19 @@ k_label_join(const typename T::type* __restrict__ logits, int classes, int64_t r
 // latter bounds the k-th largest logit from below, the k-th largest of the groups' maxima above that bound
 // does so closer; only the groups that reach it are read again, about k of them.
 struct TopSpace {
-    static constexpr int kGt = 512, kEq = 128, kFew = 256;
-    Candidates<kGt, kEq> c;
+    static constexpr int kFew = 256;
+    Candidates<512> c;
     float sup[64], val[kFew];
     uint16_t list[kFew];
     uint32_t n, kth, tot[4];
-    __device__ __forceinline__ void clear() { n = c.n_gt = c.n_eq = 0; }   // one thread, before a barrier
+    __device__ __forceinline__ void clear() { n = c.n = 0; }   // one thread, before a barrier
 };
 
-// 256 threads; m.sup and the maxima are written, with a barrier behind them
-template <class T, class F>
-__device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int parts, int part, const Vectors<T>& z,
-                                           const typename T::type* zr, int k, F emit) {
+// 256 threads; m.sup and the maxima are written, with a barrier behind them.  mine: the maxima of groups
+// 256 e + thread.
+template <class T, int M, class F>
+__device__ __forceinline__ void top_of_row(TopSpace& m, const float (&mine)[M], const float* maxima, int parts, int part,
+                                           const Vectors<T>& z, const typename T::type* zr, int k, F emit) {
     constexpr int kFew = TopSpace::kFew, W = 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = parts * 64;
     if (wave == 0) {
@@ -708,17 +720,18 @@ __device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int
     }
     __syncthreads();
     float kth = key_value(m.kth);
-    for (int i = tid; i < groups; i += 256) {
-        const float v = maxima[i];
-        if (v >= kth) {
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        const int i = e * 256 + tid;
+        if (mine[e] >= kth && i < groups) {
             const uint32_t p = atomicAdd(&m.n, 1u);
-            if (p < kFew) m.val[p] = v, m.list[p] = (uint16_t)i;
+            if (p < kFew) m.val[p] = mine[e], m.list[p] = (uint16_t)i;
         }
     }
     __syncthreads();
     const int listed = (int)m.n;
-    // with very many groups at the bound (rows mostly masked, or all equal) those that are only at it are
-    // left to first_equal
+    // with very many groups at the bound (rows mostly masked, or all equal) only those above it are read, and
+    // the first classes at it looked for
     const bool flood = listed > kFew;
     if (listed > 2 * k && !flood) {   // a closer bound
         if (wave == 0) {
@@ -732,41 +745,52 @@ __device__ __forceinline__ void top_of_row(TopSpace& m, const float* maxima, int
         kth = key_value(m.kth);
     }
     // two groups at a time per wave, one vector per lane, four reads on their way
-    constexpr int R = 4;
-    const int per = (part + 255) / 256, some = flood ? groups : listed;
-    for (int i0 = wave * 2 + (lane >> 5); i0 < some; i0 += 2 * W * R) {
-        uint4 q[R];
-        int at[R];
+    const auto collect = [&](float bound) {
+        constexpr int R = 4;
+        const int per = (part + 255) / 256, some = flood ? groups : listed;
+        for (int i0 = wave * 2 + (lane >> 5); i0 < some; i0 += 2 * W * R) {
+            uint4 q[R];
+            int at[R];
 #pragma unroll
-        for (int e = 0; e < R; ++e) {
-            const int i = i0 + e * 2 * W, v = lane & 31;
-            at[e] = -1;
-            if (i < some) {
-                const int id = flood ? i : m.list[i];
-                const float top = flood ? maxima[id] : m.val[i];
-                const int in = (v >> 2) * 256 + (id & 63) * 4 + (v & 3), u = (id >> 6) * part + in;
-                if ((flood ? top > kth : top >= kth) && (v >> 2) < per && in < part && u < z.count) at[e] = u;
+            for (int e = 0; e < R; ++e) {
+                const int i = i0 + e * 2 * W, v = lane & 31;
+                at[e] = -1;
+                if (i < some) {
+                    const int id = flood ? i : m.list[i];
+                    const float top = flood ? maxima[id] : m.val[i];
+                    const int in = (v >> 2) * 256 + (id & 63) * 4 + (v & 3), u = (id >> 6) * part + in;
+                    if (top >= bound && (v >> 2) < per && in < part && u < z.count) at[e] = u;
+                }
+                q[e] = z.load_near(at[e] < 0 ? 0 : at[e]);
             }
-            q[e] = z.load_near(at[e] < 0 ? 0 : at[e]);
-        }
 #pragma unroll
-        for (int e = 0; e < R; ++e)
-            if (at[e] >= 0) m.c.push_vector(z, at[e], z.whole(at[e]) ? q[e] : z.load_edge(at[e]), kth);
+            for (int e = 0; e < R; ++e)
+                if (at[e] >= 0) m.c.push_vector(z, at[e], z.whole(at[e]) ? q[e] : z.load_edge(at[e]), bound);
+        }
+        __syncthreads();
+        return (int)m.c.n;
+    };
+    bool strict = flood;
+    int all = collect(strict ? above(kth) : kth);
+    if (!strict && all > m.c.kMost) {
+        strict = true;
+        __syncthreads();
+        if (tid == 0) m.c.n = 0;
+        __syncthreads();
+        all = collect(above(kth));
     }
-    __syncthreads();
-    const int gt = (int)m.c.n_gt;
-    int eq = gt >= k ? 0 : (int)m.c.n_eq;
-    if (gt > TopSpace::kGt) return largest_by_passes<T, 256>(zr, z.classes, k, m.c.gt, emit);
-    if (gt < k && (flood || eq > TopSpace::kEq)) {
-        eq = 0;
-        for (int p = 0; p < parts && eq < k - gt; ++p) {
+    if (all > m.c.kMost) return largest_by_passes<T, 256>(zr, z.classes, k, m.c.key, emit);
+    if (strict && all < k) {
+        int more = 0;
+        for (int p = 0; p < parts && more < k - all; ++p) {
             if (!__any(maxima[p * 64 + lane] >= kth)) continue;
             const int from = z.first_class(p * part), to = z.first_class((p + 1) * part);
-            eq = first_equal<T, 256>(zr, from < 0 ? 0 : from, to < z.classes ? to : z.classes, kth, k - gt, eq, m.c.eq,
-                                     m.tot);
+            more = first_equal<T, 256>(zr, from < 0 ? 0 : from, to < z.classes ? to : z.classes, kth, k - all, more,
+                                       m.c.key + all, m.tot);
         }
+        all += more;
     }
-    if (wave == 0) m.c.sort(gt, eq, k, emit);
+    if (wave == 0) m.c.sort(all, k, emit);
 }
 
 // a thread's maximum to its four neighbours', and those of a workgroup's 64 fours to `to`
@@ -786,9 +810,15 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
     const typename T::type* zr = logits + row * row_stride;
     const float* mine = maxima + row * splits * 64;
     if (threadIdx.x == 0) s_m.clear();
-    float g = -kInf;
-    for (int i = threadIdx.x; i < splits * 64; i += 256) g = fmaxf(g, mine[i]);
-    put_fours(g, s_m.sup);
+    float g[kSplits / 4], top = -kInf;   // all on their way at once
+#pragma unroll
+    for (int e = 0; e < kSplits / 4; ++e) {
+        const int i = e * 256 + threadIdx.x;
+        g[e] = i < splits * 64 ? mine[i] : -kInf;
+    }
+#pragma unroll
+    for (int e = 0; e < kSplits / 4; ++e) top = fmaxf(top, g[e]);
+    put_fours(top, s_m.sup);
     const Row r = join_sums<T>(sums, zr, row, classes, labels, ignore, splits, out);
     const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
     if (r.bad()) {
@@ -796,7 +826,7 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
         return;
     }
     __syncthreads();
-    top_of_row<T>(s_m, mine, splits, part, Vectors<T>(zr, classes), zr, k, emit);
+    top_of_row<T>(s_m, g, mine, splits, part, Vectors<T>(zr, classes), zr, k, emit);
 }
 
 // Many long rows: a workgroup goes through a row alone, kPart vectors at a time, each thread with a running
@@ -819,6 +849,8 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
     const typename T::type* zr = logits + row * row_stride;
     const Vectors<T> z(zr, classes);
     if (tid == 0) s_m.clear();
+    const int64_t y = labels[row];
+    const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
     constexpr float kLow = -0x1p126f;
     float m = -kInf, ml = kLow * kL, s = 0.f, t = 0.f;
 #pragma unroll 1
@@ -879,17 +911,17 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
     s = (s_sum[0].x + s_sum[1].x) + (s_sum[2].x + s_sum[3].x);
     t = (s_sum[0].y + s_sum[1].y) + (s_sum[2].y + s_sum[3].y);
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
-    if (tid == 0) {
-        const int64_t y = labels[row];
-        put_row(out, r, row, s, t, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
-    }
+    if (tid == 192) put_row(out, r, row, s, t, zy, y, ignore, classes);   // (the first wave has more to do)
     if (k == 0) return;
     const auto emit = [&](int i, uint64_t key) { put_top(out, r, row * k + i, key); };
     if (r.bad()) {
         if (tid < k) emit(tid, 0);
         return;
     }
-    top_of_row<T>(s_m, s_max, parts, kPart, z, zr, k, emit);
+    float g[kRowParts / 4];
+#pragma unroll
+    for (int e = 0; e < kRowParts / 4; ++e) g[e] = e * 4 < parts ? s_max[e * 256 + tid] : -kInf;   // (parts * 64 of them written)
+    top_of_row<T>(s_m, g, s_max, parts, kPart, z, zr, k, emit);
 }
 
 // Few classes: one thread per row, the workgroup's rows staged through LDS as f32 (an odd pitch:
