@@ -26,7 +26,8 @@ namespace {
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kL = 1.44269504f, kLn2 = 0.693147182f;
 constexpr float kFloor = -1000.f;            // 2^x is 0 well above
-constexpr int kSmall = 64;                   // most classes of the kernels of one thread per row
+// most classes of the kernels of one thread per row (300000 x 64 f32 with 3 alternatives: 38 us, sixteen lanes 51)
+constexpr int kSmall = 64;
 constexpr int kSplits = 64;                  // most parts of a row
 
 inline hipStream_t as_stream(void* s) { return (hipStream_t)s; }
@@ -106,10 +107,6 @@ __device__ __forceinline__ uint4 load16(const typename T::type* p) {
     __builtin_memcpy(&q, p, 16);
     return q;
 }
-template <class T>
-__device__ __forceinline__ void store16(typename T::type* p, const uint4& q) {
-    __builtin_memcpy(p, &q, 16);
-}
 // the elements [from, to) of sixteen bytes, from < to, the others -inf (all reads on their way at once: in
 // the others' places the nearest element is read)
 template <class T>
@@ -127,7 +124,7 @@ __device__ __forceinline__ uint4 load_some(const typename T::type* p, int from, 
 
 // A row as aligned vectors of 16 bytes: vector u holds the classes u V - skip and on.  Its first and
 // last vector may be partly other rows'.  (Rows of an odd number of 16-bit classes, read at their own
-// alignment: 66 us for 2048 x 50021 bf16; in aligned vectors 48.)
+// alignment: 66 us for 2048 x 50021 bf16; in aligned vectors 43.)
 template <class T>
 struct Vectors {
     const typename T::type* base;
@@ -621,9 +618,8 @@ k_label_lanes(const typename T::type* __restrict__ logits, int64_t n, int classe
 // vectors (four neighbouring threads' each).
 template <class T, int NCH>
 __global__ void __launch_bounds__(256, 8)
-k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t row_stride,
-             const int64_t* __restrict__ labels, int64_t ignore, int splits, int part, Out out, float4* __restrict__ sums,
-             float* __restrict__ maxima) {
+k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t row_stride, int splits, int part,
+             float4* __restrict__ sums, float* __restrict__ maxima) {
     __shared__ float s_max[4];
     __shared__ float2 s_sum[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -661,13 +657,7 @@ k_label_part(const typename T::type* __restrict__ logits, int classes, int64_t r
     if (tid != 0) return;
     s = (s_sum[0].x + s_sum[1].x) + (s_sum[2].x + s_sum[3].x);
     t = (s_sum[0].y + s_sum[1].y) + (s_sum[2].y + s_sum[3].y);
-    if (sums) {
-        sums[blockIdx.x] = make_float4(r.m, s, t, 0.f);
-        return;
-    }
-    r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
-    const int64_t y = labels[row];
-    put_row(out, r, row, s, t, y >= 0 && y < classes ? T::one(zr + y) : 0.f, y, ignore, classes);
+    sums[blockIdx.x] = make_float4(r.m, s, t, 0.f);
 }
 
 // The parts' sums taken to the row's maximum (one lane per part, every wave alike).
@@ -832,8 +822,10 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
 // Many long rows: a workgroup goes through a row alone, kPart vectors at a time, each thread with a running
 // maximum of its own (2^x is taken to it, and what it has summed is taken to a new one), so nothing waits
 // for the other threads before the row's end.
-constexpr int kPart = 256 * 4;     // vectors of a part
-static_assert((PIN_LABEL_CLASSES_MAX + 6) / 4 <= (int64_t)kSplits * 2 * kPart, "the longest row's parts");
+// vectors of a part (of twice as many: 2048 x 50021 bf16 47 us instead of 44, 4096 x 131072 alike)
+constexpr int kPart = 256 * 4;
+static_assert((PIN_LABEL_CLASSES_MAX + 6) / 4 <= kSplits * 2 * kPart && (PIN_LABEL_CLASSES_MAX + 14) / 8 <= kSplits * kPart,
+              "the longest row's parts");
 constexpr int kRowParts = 32;      // most parts of a row here (their groups' maxima lie in LDS)
 
 template <class T>
@@ -927,7 +919,7 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
 // Few classes: one thread per row, the workgroup's rows staged through LDS as f32 (an odd pitch:
 // consecutive rows begin in different banks).  Rows without gaps are read as vectors, eight on their way
 // per thread (1M x 20 f32 with 3 alternatives: element by element 65 us, in vectors and with the row in
-// registers 36).
+// registers 30).
 template <class T, int ROWS>
 __device__ __forceinline__ void stage_rows(const typename T::type* __restrict__ logits, int64_t row0, int rows, int classes,
                                            uint32_t magic, int64_t row_stride, float* s_z) {
@@ -1323,23 +1315,25 @@ int forward_rows(const Call& a, const Plan& p) {
                            a.labels, a.ignore, a.k, p.alone, a.out);
         return launch_status();
     }
-    const bool join = p.splits > 1 || a.k > 0;
-    if (join && (!a.ws || ((uintptr_t)a.ws & 15))) return PIN_ERR_ARG;
-    float4* sums = join ? (float4*)a.ws : nullptr;
+    if (!a.ws || ((uintptr_t)a.ws & 15)) return PIN_ERR_ARG;
+    float4* sums = (float4*)a.ws;
     float* maxima = a.k > 0 ? (float*)(sums + a.n * p.splits) : nullptr;
     const dim3 grid((unsigned)(a.n * p.splits)), rows((unsigned)a.n);
-    if (p.part <= kPart)
-        hipLaunchKernelGGL((k_label_part<T, 4>), grid, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
-                           a.ignore, p.splits, p.part, a.out, sums, maxima);
-    else
-        hipLaunchKernelGGL((k_label_part<T, 8>), grid, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
-                           a.ignore, p.splits, p.part, a.out, sums, maxima);
+    const auto parts = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, p.splits, p.part, sums, maxima);
+    };
+    if constexpr (T::N == F32::N) {   // (the longest rows of 16-bit classes fit kSplits parts of kPart)
+        if (p.part > kPart) parts(k_label_part<T, 8>);
+        else parts(k_label_part<T, 4>);
+    } else {
+        parts(k_label_part<T, 4>);
+    }
     if (a.k > 0)
         hipLaunchKernelGGL((k_label_join_top<T>), rows, dim3(256), 0, a.st, z, (int)a.classes, a.row_stride, a.labels,
                            a.ignore, a.k, p.splits, p.part, a.out, sums, maxima);
-    else if (join)
-        hipLaunchKernelGGL((k_label_join<T>), dim3((unsigned)a.n), dim3(64), 0, a.st, z, (int)a.classes, a.row_stride,
-                           a.labels, a.ignore, p.splits, a.out, sums);
+    else
+        hipLaunchKernelGGL((k_label_join<T>), rows, dim3(64), 0, a.st, z, (int)a.classes, a.row_stride, a.labels, a.ignore,
+                           p.splits, a.out, sums);
     return launch_status();
 }
 
@@ -1380,7 +1374,9 @@ int backward_rows(const Call& a, const int64_t* top_idx, const float* stats, con
                                u, o);
         return launch_status();
     }
-    const int lanes = a.classes <= 16 * T::N * 4 && a.k < 16 ? 16 : a.classes <= 64 * T::N * 8 ? 64 : 256;
+    // sixteen lanes per row (and one more than k): 16384 x 1003 f16 with 8 alternatives 18 us, 64 lanes 22;
+    // 64 lanes up to 64 * 8 vectors: 16384 x 3000 bf16 45 us, a workgroup 49
+    const int lanes = a.classes <= 16 * T::N * 8 && a.k < 16 ? 16 : a.classes <= 64 * T::N * 8 ? 64 : 256;
     const int64_t vecs = (a.classes + 2 * T::N - 2) / T::N;
     const int part = lanes == 256 ? 256 * 4 : (int)vecs;
     const int64_t parts = (vecs + part - 1) / part;
@@ -1424,7 +1420,7 @@ int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dt
         return PIN_ERR_ARG;
     if (n == 0 || classes <= kSmall) return 0;
     const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N, top_k);
-    return p.lanes > 0 || p.nch > 0 || p.alone > 0 || (p.splits == 1 && top_k == 0) ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
+    return p.lanes > 0 || p.nch > 0 || p.alone > 0 ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
 }
 
 int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,
