@@ -109,11 +109,10 @@ class AdamW(torch.optim.Optimizer):
         if not self.capturable or lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device:
             raise ValueError("AdamW: a tensor lr must be one float32 on the parameters' device, with capturable=True")
 
-    def _check_group(self, group):
+    @staticmethod
+    def _check_rates(group):
         lr, (b1, b2) = group["lr"], group["betas"]
-        if isinstance(lr, torch.Tensor):
-            self._check_lr(lr, group["params"][0].device)
-        elif not 0.0 <= lr < float("inf"):
+        if not 0.0 <= lr < float("inf"):
             raise ValueError(f"AdamW: lr must be >= 0 (got {lr})")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW: betas must be in [0, 1) (got {group['betas']})")
@@ -121,7 +120,14 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: eps and weight_decay must be >= 0 (got {group['eps']}, {group['weight_decay']})")
         if group["state_bits"] not in _STATE_KEYS:
             raise ValueError(f"AdamW: state_bits must be 32 or 8 (got {group['state_bits']})")
+
+    def _check_group(self, group):
         params = group["params"]
+        if isinstance(group["lr"], torch.Tensor):
+            self._check_lr(group["lr"], params[0].device)
+            self._check_rates({**group, "lr": 0.0})
+        else:
+            self._check_rates(group)
         spans = []
         for p in params:
             if p.dtype not in _lib.TYPES:
@@ -295,6 +301,7 @@ class AdamW(torch.optim.Optimizer):
             for key in ("state_bits", "master_weights"):
                 if mine[key] != saved[key]:
                     raise ValueError(f"AdamW: the saved state has {key} {saved[key]}, this optimiser {mine[key]}")
+            self._check_rates({**saved, "lr": float(saved["lr"])})
         plan = []
         k = 0
         for gi, group in enumerate(self.param_groups):
@@ -320,8 +327,10 @@ class AdamW(torch.optim.Optimizer):
         self._arenas.clear()
         self.state.clear()
         for mine, saved in zip(self.param_groups, groups):
-            mine.update({key: val for key, val in saved.items() if key != "params"})
-            self._check_group(mine)
+            lr = float(saved["lr"])
+            if isinstance(mine["lr"], torch.Tensor):   # (a graph may read it)
+                lr = mine["lr"].fill_(lr)
+            mine.update({key: val for key, val in saved.items() if key != "params"}, lr=lr)
         to, by = {}, {}
         for gi, i, p, want, one in plan:
             arena = self._arena(gi)

@@ -349,6 +349,10 @@ def test_load_refuses_what_does_not_fit(dev):
         P.AdamW(tensors([300, 2], torch.float32, dev), state_bits=8).load_state_dict(saved)
     with pytest.raises(ValueError, match="exp_avg"):
         P.AdamW(tensors([301], torch.float32, dev), state_bits=8).load_state_dict(saved)
+    worse = {**saved, "param_groups": [{**saved["param_groups"][0], "betas": (0.9, 1.0)}]}
+    with pytest.raises(ValueError, match="betas"):
+        opt.load_state_dict(worse)
+    assert opt.param_groups[0]["betas"] == HYPER["betas"] and opt.state_dict()["state"][0]["step"] == 1   # as it was
     bad = copy.copy(saved)
     bad["state"] = {0: {**saved["state"][0], "exponents": saved["state"][0]["exponents"][:1]}}
     with pytest.raises(ValueError, match="exponents"):
@@ -388,6 +392,10 @@ def test_captured_and_replayed(dev, bits):
         for x, y in zip(opt.moments(), ref.moments()):
             assert torch.equal(x, y)
     assert opt.state_dict()["state"][0]["step"] == 5
+    saved = copy.deepcopy(opt.state_dict())
+    graph.replay()
+    opt.load_state_dict(saved)   # the lr's value goes to where the graph reads it
+    assert opt.param_groups[0]["lr"] is lr and opt.state_dict()["state"][0]["step"] == 5
 
 
 @pytest.mark.parametrize("bits", [32, 8])
