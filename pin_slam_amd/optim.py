@@ -18,13 +18,17 @@ import torch
 from . import _lib
 
 _ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_dtype = torch.Tensor.dtype.__get__
+_get_device, _dtype, _grad = torch.Tensor.get_device, torch.Tensor.dtype.__get__, torch.Tensor.grad.__get__
 _SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
 
 
 def _blocks(n):
     return -(-n // _lib.ADAMW_BLOCK)
+
+
+def _has_master(group):
+    return group["master_weights"] and any(p.dtype != torch.float32 for p in group["params"])
 
 
 class _Arena:
@@ -45,19 +49,32 @@ class _Arena:
         self.m = torch.zeros((total,), dtype=kind, device=dev)
         self.v = torch.zeros((total,), dtype=kind, device=dev)
         self.exps = torch.zeros((total // _lib.ADAMW_BLOCK, 2), dtype=torch.int16, device=dev) if bits == 8 else None
-        self.master = None
-        if group["master_weights"] and any(p.dtype != torch.float32 for p in params):
-            self.master = torch.zeros((total,), dtype=torch.float32, device=dev)
-            for p, a, n in zip(params, self.offsets, self.sizes):
-                self.master[a:a + n] = p.detach().reshape(-1)
-        self.steps = [0] * len(params)
-        self.together = True              # all of them are the same
+        self.master = torch.zeros((total,), dtype=torch.float32, device=dev) if _has_master(group) else None
         self.held = None
-        self.where, self.kinds = None, set()   # the parameters as they were last checked one by one
+        self.twice = self.sizes * 2
+        self.index = dev.index
         self.c_sizes, self.c_offsets = array("q", self.sizes), array("q", self.offsets)
         # a step that a graph may replay counts on the device, all of the group's parameters together
         self.step_dev = torch.zeros((1,), dtype=torch.int64, device=dev) if capturable else None
         self.scalars = torch.zeros((_lib.ADAMW_SCALARS_BYTES,), dtype=torch.uint8, device=dev) if capturable else None
+        self.start(params)
+
+    def arrays(self):
+        return [x for x in (self.m, self.v, self.exps, self.master, self.step_dev) if x is not None]
+
+    def start(self, params):
+        """As before the first step, where it lies (a captured graph goes on with it)."""
+        for x in self.arrays():
+            x.zero_()
+        if self.master is not None:
+            for p, a, n in zip(params, self.offsets, self.sizes):
+                self.master[a:a + n] = p.detach().reshape(-1)
+        self.steps = [0] * len(params)
+        self.together = True              # all of them are the same
+
+    def fits(self, group):
+        return (self.sizes == [p.numel() for p in group["params"]] and (self.master is not None) == _has_master(group)
+                and all(p.device == self.device for p in group["params"]))
 
     def views(self, i, shape):
         """The parameter's part of each array."""
@@ -173,20 +190,20 @@ class AdamW(torch.optim.Optimizer):
         """What has a gradient, checked: launches of (indexes or None for all, their type, addresses of the parameters and
         of the gradients)."""
         params = group["params"]
-        grads = [p.grad for p in params]
+        grads = list(map(_grad, params))
         if type(None) in set(map(type, grads)):
             if self.capturable:
                 raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
             which = [i for i, g in enumerate(grads) if g is not None]
         else:
-            # the usual step: every parameter where it was and as it was, every gradient as the kernel takes it.  One
-            # pass per property: for many tensors this is the step's cost on the host.
-            where = list(map(_ptr, params))
+            # the usual step: every parameter and every gradient as the kernel takes them.  One pass per property: for
+            # many tensors this is the step's cost on the host.
+            both, n, kind = params + grads, len(params), params[0].dtype
             try:
-                if (where == arena.where and arena.together and list(map(_numel, params)) == arena.sizes
-                        and list(map(_numel, grads)) == arena.sizes and set(map(_dtype, grads)) == arena.kinds
-                        and len(arena.kinds) == 1 and all(map(_contiguous, grads))):
-                    return [(None, params[0].dtype, where, list(map(_ptr, grads)))]
+                if (arena.together and kind in _lib.TYPES and list(map(_numel, both)) == arena.twice
+                        and list(map(_dtype, both)).count(kind) == 2 * n
+                        and list(map(_get_device, both)).count(arena.index) == 2 * n and all(map(_contiguous, both))):
+                    return [(None, kind, array("Q", map(_ptr, params)), array("Q", map(_ptr, grads)))]
             except RuntimeError:   # a sparse one has no contiguity and no address
                 pass
             which = range(len(params))
@@ -194,13 +211,11 @@ class AdamW(torch.optim.Optimizer):
         held = arena.held = []   # copies made here live until the step is on its way
         for i in which:
             g = self._check(arena, i, params[i], grads[i])
-            idx, ps, gs = some.setdefault((params[i].dtype, arena.steps[i]), ([], [], []))
+            idx, ps, gs = some.setdefault((params[i].dtype, arena.steps[i]), ([], array("Q"), array("Q")))
             idx.append(i)
             ps.append(params[i].data_ptr())
             gs.append(g.data_ptr())
             held.append(g)
-        if len(which) == len(params):
-            arena.where, arena.kinds = [p.data_ptr() for p in params], {p.dtype for p in params}
         return [(idx, dtype, ps, gs) for (dtype, _), (idx, ps, gs) in some.items()]
 
     @torch.no_grad()
@@ -244,7 +259,6 @@ class AdamW(torch.optim.Optimizer):
                 n = len(idx)
                 sizes, offsets = (array("q", [x[i] for i in idx]) for x in (arena.sizes, arena.offsets))
             t = arena.steps[0 if idx is None else idx[0]] + (0 if self.capturable else 1)
-            ps, gs = array("Q", ps), array("Q", gs)
             master = arena.master if dtype != torch.float32 else None
             _lib.call("pin_adamw_step", *(x.buffer_info()[0] for x in (ps, gs, sizes, offsets)), n, _lib.TYPES[dtype],
                       arena.bits, _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total,
@@ -293,7 +307,8 @@ class AdamW(torch.optim.Optimizer):
         return saved
 
     def load_state_dict(self, state_dict):
-        """Takes a state_dict of an AdamW with the same groups (its state_bits and master_weights too)."""
+        """Takes a state_dict of an AdamW with the same groups (its state_bits and master_weights too).  State that is
+        there already is written where it lies, so a graph that holds a step goes on from what was loaded."""
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the saved state has other parameter groups")
@@ -310,9 +325,7 @@ class AdamW(torch.optim.Optimizer):
                 k += 1
                 if one is None:
                     continue
-                want = [*_STATE_KEYS[group["state_bits"]]]
-                if group["master_weights"] and any(q.dtype != torch.float32 for q in group["params"]):
-                    want.append("master")
+                want = [*_STATE_KEYS[group["state_bits"]]] + ["master"] * _has_master(group)
                 kind = torch.float32 if group["state_bits"] == 32 else torch.uint8
                 for key in want:
                     shape = (_blocks(p.numel()), 2) if key == "exponents" else tuple(p.shape)
@@ -324,8 +337,20 @@ class AdamW(torch.optim.Optimizer):
                 plan.append((gi, i, p, want, one))
             if self.capturable and len({int(o["step"]) for g, _, _, _, o in plan if g == gi}) > 1:
                 raise ValueError("AdamW: with capturable=True the parameters of a group share one step")
-        self._arenas.clear()
-        self.state.clear()
+        # the optimiser's own state_dict is views of what is started anew here
+        own = {x.untyped_storage().data_ptr() for arena in self._arenas.values() for x in arena.arrays()}
+        plan = [(gi, i, p, want, {key: x.clone() if key in want and x.untyped_storage().data_ptr() in own else x
+                                  for key, x in one.items()}) for gi, i, p, want, one in plan]
+        for gi, group in enumerate(self.param_groups):
+            arena = self._arenas.get(gi)
+            if arena is None:
+                continue
+            if arena.fits(group):
+                arena.start(group["params"])
+            else:
+                del self._arenas[gi]
+                for p in group["params"]:
+                    self.state.pop(p, None)
         for mine, saved in zip(self.param_groups, groups):
             lr = float(saved["lr"])
             if isinstance(mine["lr"], torch.Tensor):   # (a graph may read it)

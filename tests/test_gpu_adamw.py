@@ -398,6 +398,57 @@ def test_captured_and_replayed(dev, bits):
     assert opt.param_groups[0]["lr"] is lr and opt.state_dict()["state"][0]["step"] == 5
 
 
+@pytest.mark.parametrize("bits,kind", [(32, torch.bfloat16), (8, torch.float32)])
+def test_a_captured_step_goes_on_from_what_was_loaded(dev, bits, kind):
+    """Loading writes the state where it lies: replays after it equal steps of an optimiser that loaded the same."""
+    a, b = tensors([5000, 257], kind, dev), tensors([5000, 257], kind, dev)
+    new = lambda p: P.AdamW(p, state_bits=bits, master_weights=True, capturable=True, **HYPER)   # noqa: E731
+    opt, ref = new(a), new(b)
+    set_grads(a, 0)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    saved, at = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in a]
+    graph.replay()
+    spare = [torch.full((5000,), float("nan"), device=dev) for _ in range(8)]   # (what a freed state would become)
+    for own in (False, True):
+        opt.load_state_dict(opt.state_dict() if own else saved)   # its own, views of its state, changes nothing
+        if own:
+            graph.replay()
+            ref.step()
+        else:
+            ref.load_state_dict(saved)
+            with torch.no_grad():
+                for p, q, x in zip(a, b, at):
+                    p.copy_(x)
+                    q.copy_(x)
+            set_grads(b, 0)
+            graph.replay()
+            ref.step()
+        torch.cuda.synchronize()
+        for p, q in zip([*a, *opt.moments()], [*b, *ref.moments()]):
+            assert torch.equal(p, q)
+    assert opt.state_dict()["state"][1]["step"] == ref.state_dict()["state"][1]["step"] == 4
+    assert all(bool(x.isnan().all()) for x in spare)
+    opt.load_state_dict(new(tensors([5000, 257], kind, dev)).state_dict())   # one that never stepped
+    assert not any(bool(x.any()) for x in opt.moments()) and opt.state_dict()["state"][0]["step"] == 0
+
+
+def test_a_parameter_laid_out_anew_is_refused(dev):
+    p = tensors([64 * 64], torch.float32, dev)[0]
+    p.data = p.data.view(64, 64)
+    opt = P.AdamW([p], **HYPER)
+    for _ in range(2):
+        p.grad = torch.ones(64, 64, device=dev)
+        opt.step()
+    p.data = p.data.t()   # the same address and size, the gradient as before
+    with pytest.raises(RuntimeError, match="reshaped"):
+        opt.step()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_copied_with_its_parameters(dev, bits):
     a = tensors([1000, 33], torch.float32, dev)
