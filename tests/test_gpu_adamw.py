@@ -584,6 +584,45 @@ def test_a_training_step_of_the_class_head(dev):
         assert float((x - y).abs().max()) <= 0.1 * 5 * 0.01
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_training_step(dev, bits):
+    """Loss, gradient into the leaf's own .grad and step in one graph, replayed between eager work, against the same calls
+    made eagerly."""
+    n, c = 300, 700
+    labels = [torch.randint(0, c, (n,), generator=torch.Generator().manual_seed(t)).to(dev) for t in range(5)]
+    up = torch.full((n,), -1.0 / n, device=dev)
+
+    def start():
+        x = torch.nn.Parameter(torch.randn((n, c), generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(dev))
+        return x, P.AdamW([x], state_bits=bits, master_weights=True, capturable=True, **HYPER)
+
+    def turn(x, opt, y):
+        x.grad = None
+        r = P.label_log_probs(x, y, top_k=2)
+        torch.autograd.backward([r.log_prob, r.entropy], [up, up])
+        opt.step()
+        return r.log_prob.detach(), r.top_index
+
+    (x, opt), (q, ref) = start(), start()
+    y = labels[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        turn(x, opt, y)
+    torch.cuda.current_stream().wait_stream(side)
+    turn(q, ref, labels[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = turn(x, opt, y)
+    for t in range(1, 5):
+        y.copy_(labels[t])
+        want = turn(q, ref, labels[t])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([*out, x, x.grad, *opt.moments(), opt.master()],
+                                                     [*want, q, q.grad, *ref.moments(), ref.master()]))
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
