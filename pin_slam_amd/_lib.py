@@ -12,6 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PIN_LIB overrides the library path (experiment variants built by tools/variants.py)
 LIB_PATH = os.environ.get("PIN_LIB") or os.path.join(_HERE, "libpin_slam_amd.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "libpin_slam_torch.so")
 
 PIN_OK = 0
 PIN_TRAIN_ROWS = 1   # PinTrainCfg.flags: coord holds every row of the iteration
@@ -242,6 +243,7 @@ _RESTYPES = {"pin_map_workspace_bytes": i64, "pin_mc_workspace_bytes": i64,
              "pin_pool_window_workspace_bytes": i64, "pin_label_logprob_workspace_bytes": i64}
 
 _lib = None
+_gather = None
 
 
 def exported_symbols():
@@ -263,6 +265,24 @@ def load():
         fn.restype = _RESTYPES.get(name, ctypes.c_int)
     _lib = lib
     return lib
+
+
+def torch_gather():
+    """pin_torch_gather of the library that is built against torch (csrc/pin_torch.cpp)."""
+    global _gather
+    if _gather is None:
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise RuntimeError(f"pin_slam_amd: native library not built ({TORCH_LIB_PATH}); run "
+                               "`python -m pin_slam_amd.build` or __graft_entry__.build().")
+        lib = ctypes.PyDLL(TORCH_LIB_PATH)
+        lib.pin_torch_version.restype = ctypes.c_char_p
+        built = lib.pin_torch_version().decode()
+        if built.split("+")[0] != torch.__version__.split("+")[0]:
+            raise RuntimeError(f"pin_slam_amd: {TORCH_LIB_PATH} was built for torch {built}, this is {torch.__version__}")
+        lib.pin_torch_gather.argtypes = [ctypes.py_object, i64, c_void_p, i64, c_void_p, c_void_p]
+        lib.pin_torch_gather.restype = ctypes.c_int
+        _gather = lib.pin_torch_gather
+    return _gather
 
 
 def call(name, *args):

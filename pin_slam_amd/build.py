@@ -1,4 +1,5 @@
-"""Build the gfx950 shared library in-tree: pin_slam_amd/libpin_slam_amd.so.
+"""Build the gfx950 shared library in-tree, pin_slam_amd/libpin_slam_amd.so, and beside it
+libpin_slam_torch.so (csrc/pin_torch.cpp, host code against torch's headers).
 
 hipcc cross-compiles for gfx950 without a GPU, so this runs in the build
 container; the resulting .so travels to the GPU box with the repo snapshot.
@@ -8,11 +9,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libpin_slam_amd.so")
+TORCH_LIB = os.path.join(HERE, "libpin_slam_torch.so")
+TORCH_SOURCE = os.path.join(HERE, "csrc", "pin_torch.cpp")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
@@ -31,11 +35,21 @@ def sources():
 
 
 def _stale():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
         return True
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(HERE, "csrc", "*.h")) + [os.path.join(ROOT, "include", "pin_slam_amd.h")]
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
+    deps = sources() + glob.glob(os.path.join(HERE, "csrc", "*.h")) + [TORCH_SOURCE, os.path.join(ROOT, "include", "pin_slam_amd.h")]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _torch_command(out):
+    import torch
+    from torch.utils import cpp_extension
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+            *[f"-isystem{p}" for p in cpp_extension.include_paths()], f"-isystem{sysconfig.get_paths()['include']}",
+            TORCH_SOURCE, f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", out]
 
 
 def build(force: bool = False, verbose: bool = False, extra=(), out: str = None) -> str:
@@ -50,6 +64,11 @@ def build(force: bool = False, verbose: bool = False, extra=(), out: str = None)
     try:
         procs = []
         objs = []
+        if out == LIB:
+            cmd = _torch_command(TORCH_LIB + ".tmp")
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            procs.append((cmd, subprocess.Popen(cmd)))
         for src in sources():
             obj = os.path.join(objdir, os.path.basename(src) + ".o")
             cmd = [HIPCC, *[f for f in FLAGS if f != "-shared"], *extra, *inc, "-c", src, "-o", obj]
@@ -64,6 +83,8 @@ def build(force: bool = False, verbose: bool = False, extra=(), out: str = None)
     finally:
         shutil.rmtree(objdir, ignore_errors=True)
     os.replace(out + ".tmp", out)
+    if out == LIB:
+        os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
     return out
 
 

@@ -17,8 +17,6 @@ import torch
 
 from . import _lib
 
-_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_get_device, _dtype, _grad = torch.Tensor.get_device, torch.Tensor.dtype.__get__, torch.Tensor.grad.__get__
 _SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
 
@@ -51,7 +49,6 @@ class _Arena:
         self.exps = torch.zeros((total // _lib.ADAMW_BLOCK, 2), dtype=torch.int16, device=dev) if bits == 8 else None
         self.master = torch.zeros((total,), dtype=torch.float32, device=dev) if _has_master(group) else None
         self.held = None
-        self.twice = self.sizes * 2
         self.index = dev.index
         self.c_sizes, self.c_offsets = array("q", self.sizes), array("q", self.offsets)
         # a step that a graph may replay counts on the device, all of the group's parameters together
@@ -190,23 +187,16 @@ class AdamW(torch.optim.Optimizer):
         """What has a gradient, checked: launches of (indexes or None for all, their type, addresses of the parameters and
         of the gradients)."""
         params = group["params"]
-        grads = list(map(_grad, params))
-        if type(None) in set(map(type, grads)):
-            if self.capturable:
-                raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
-            which = [i for i, g in enumerate(grads) if g is not None]
-        else:
-            # the usual step: every parameter and every gradient as the kernel takes them.  One pass per property: for
-            # many tensors this is the step's cost on the host.
-            both, n, kind = params + grads, len(params), params[0].dtype
-            try:
-                if (arena.together and kind in _lib.TYPES and list(map(_numel, both)) == arena.twice
-                        and list(map(_dtype, both)).count(kind) == 2 * n
-                        and list(map(_get_device, both)).count(arena.index) == 2 * n and all(map(_contiguous, both))):
-                    return [(None, kind, array("Q", map(_ptr, params)), array("Q", map(_ptr, grads)))]
-            except RuntimeError:   # a sparse one has no contiguity and no address
-                pass
-            which = range(len(params))
+        n = len(params)
+        if arena.together:   # the usual step: every parameter and every gradient as the kernel takes them
+            ps, gs = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
+            if _lib.torch_gather()(params, n, arena.c_sizes.buffer_info()[0], arena.index, ps.buffer_info()[0],
+                                   gs.buffer_info()[0]) >= 0:
+                return [(None, params[0].dtype, ps, gs)]
+        grads = [p.grad for p in params]
+        which = [i for i, g in enumerate(grads) if g is not None]
+        if self.capturable and len(which) < n:
+            raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient")
         some = {}
         held = arena.held = []   # copies made here live until the step is on its way
         for i in which:

@@ -105,3 +105,62 @@ def test_argument_errors_before_any_device_work():
     assert lib.pin_adamw_moments(ok, ok, ok, 100, ok, ok, None) == -1
     assert lib.pin_adamw_moments(ok, ok, None, 256, ok, ok, None) == -1
     assert lib.pin_adamw_moments(ok, ok, ok, 0, None, None, None) == 0
+
+
+def test_addresses_of_many_tensors():
+    """pin_torch_gather: addresses of what is as the kernel takes it, refusal of anything else (host tensors, device -1)."""
+    import weakref
+    from array import array
+
+    gather = _lib.torch_gather()
+
+    def make(kind=torch.float32, shapes=((7,), (3, 4), (), (0,))):
+        out = [torch.nn.Parameter(torch.ones(s, dtype=kind)) for s in shapes]
+        for p in out:
+            p.grad = torch.zeros_like(p)
+        return out
+
+    def ask(params, sizes=None, device=-1):
+        sizes = array("q", [p.numel() for p in params] if sizes is None else sizes)
+        n = len(sizes)
+        ps, gs = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
+        return gather(params, n, *(x if isinstance(x, int) else x.buffer_info()[0] for x in (sizes, device, ps, gs))), ps, gs
+
+    for kind, code in _lib.TYPES.items():
+        params = make(kind)
+        rc, ps, gs = ask(params)
+        assert rc == code
+        assert list(ps) == [p.data_ptr() for p in params] and list(gs) == [p.grad.data_ptr() for p in params]
+    assert ask(make(torch.float64))[0] == -1
+    assert ask(make(), device=0)[0] == -1
+    assert ask(make(), sizes=[7, 12, 1, 1])[0] == -1 and ask(make(), sizes=[7, 12, 1])[0] == -1
+    assert ask([])[0] == -1 and ask(tuple(make()), sizes=[7, 12, 1, 0])[0] == -1
+    assert ask([*make(), 3], sizes=[7, 12, 1, 0, 1])[0] == -1
+
+    def changed(i, f):
+        params = make(shapes=((7,), (4, 4)))
+        f(params[i])
+        return ask(params, sizes=[7, 16])[0]
+
+    assert changed(0, lambda p: None) == 0
+    assert changed(0, lambda p: setattr(p, "grad", None)) == -1
+    assert changed(1, lambda p: setattr(p, "data", p.data.t())) == -1
+    assert changed(1, lambda p: setattr(p, "grad", torch.zeros(4, 4).t())) == -1
+    assert changed(1, lambda p: setattr(p, "data", torch.ones(4, 4, dtype=torch.float16))) == -1
+    assert changed(1, lambda p: setattr(p, "grad", torch.zeros(4, 4).to_sparse())) == -1
+    m = torch.nn.Parameter(torch.ones(7, device="meta"))
+    m.grad = torch.zeros(7, device="meta")
+    assert ask([m])[0] == -1   # no addresses
+    assert ask([*make(torch.float32), *make(torch.float16)])[0] == -1
+    p = make()[0]
+    assert ask([p * 1], sizes=[7])[0] == -1   # not a leaf
+
+    class Other(torch.Tensor):
+        pass
+
+    q = torch.nn.Parameter(torch.ones(7).as_subclass(Other))
+    q.grad = torch.zeros(7)
+    assert ask([q], sizes=[7])[0] == -1
+    gone = weakref.ref(p)   # no reference is kept
+    del p
+    assert gone() is None
