@@ -243,7 +243,7 @@ _RESTYPES = {"pin_map_workspace_bytes": i64, "pin_mc_workspace_bytes": i64,
              "pin_pool_window_workspace_bytes": i64, "pin_label_logprob_workspace_bytes": i64}
 
 _lib = None
-_gather = None
+_torch_lib = None
 
 
 def exported_symbols():
@@ -267,10 +267,16 @@ def load():
     return lib
 
 
-def torch_gather():
-    """pin_torch_gather of the library that is built against torch (csrc/pin_torch.cpp)."""
-    global _gather
-    if _gather is None:
+_TORCH_SIGS = {   # functions of the library that is built against torch (csrc/pin_torch.cpp)
+    "pin_torch_gather": [ctypes.py_object, i64, c_void_p, i64, c_void_p, c_void_p],
+    "pin_torch_label_attach": [c_void_p] + [ctypes.py_object] * 7 + [i64, i64],
+}
+
+
+def torch_fn(name):
+    """The bound entry point of the library that is built against torch."""
+    global _torch_lib
+    if _torch_lib is None:
         if not os.path.exists(TORCH_LIB_PATH):
             raise RuntimeError(f"pin_slam_amd: native library not built ({TORCH_LIB_PATH}); run "
                                "`python -m pin_slam_amd.build` or __graft_entry__.build().")
@@ -279,10 +285,21 @@ def torch_gather():
         built = lib.pin_torch_version().decode()
         if built.split("+")[0] != torch.__version__.split("+")[0]:
             raise RuntimeError(f"pin_slam_amd: {TORCH_LIB_PATH} was built for torch {built}, this is {torch.__version__}")
-        lib.pin_torch_gather.argtypes = [ctypes.py_object, i64, c_void_p, i64, c_void_p, c_void_p]
-        lib.pin_torch_gather.restype = ctypes.c_int
-        _gather = lib.pin_torch_gather
-    return _gather
+        for key, args in _TORCH_SIGS.items():
+            getattr(lib, key).argtypes = args
+            getattr(lib, key).restype = ctypes.c_int
+        _torch_lib = lib
+    return getattr(_torch_lib, name)
+
+
+_addresses = {}
+
+
+def address(name):
+    """Address of an entry point, for native code that calls it."""
+    if name not in _addresses:
+        _addresses[name] = ctypes.cast(fn(name), c_void_p)
+    return _addresses[name]
 
 
 def call(name, *args):

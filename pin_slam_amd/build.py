@@ -47,9 +47,10 @@ def _torch_command(out):
     from torch.utils import cpp_extension
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+            "-isystem/opt/rocm/include", "-I", os.path.join(ROOT, "include"),
             *[f"-isystem{p}" for p in cpp_extension.include_paths()], f"-isystem{sysconfig.get_paths()['include']}",
-            TORCH_SOURCE, f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", out]
+            TORCH_SOURCE, f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-o", out]
 
 
 def build(force: bool = False, verbose: bool = False, extra=(), out: str = None) -> str:

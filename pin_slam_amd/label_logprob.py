@@ -3,12 +3,12 @@
 The loss beside the classification heads (model/decoder.py:120: log_softmax and argmax over
 the classes): one pass over the logits gives what a training loss, a confidence and a list of
 alternatives need, and the gradient recomputes the probabilities from the logits, so nothing of
-the logits' size is kept between the two (pin_label_logprob, pin_label_logprob_bwd).
+the logits' size is kept between the two (pin_label_logprob, pin_label_logprob_bwd).  The
+gradient's node in torch's graph is native (csrc/pin_torch.cpp).
 """
 from collections import namedtuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -32,48 +32,6 @@ def _forward(z, y, k, ignore, want_stats):
               ent.data_ptr(), stats.data_ptr() if want_stats else None, tlp.data_ptr() if k else None,
               tidx.data_ptr() if k else None, None if ws is None else ws.data_ptr(), _lib.raw_stream(z.get_device()))
     return lp, ent, stats, tlp, tidx
-
-
-def _f32(g):
-    """An upstream gradient as the kernel takes it."""
-    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
-
-
-def _backward(ctx, g_lp, g_ent, g_top=None, _=None):
-    z, y, *top = ctx.saved_tensors
-    n, c = z.shape
-    k = top[0].shape[1] if top else 0
-    g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
-    dz = z.new_empty((n, c))
-    # (autograd runs this on the logits' device and the forward's stream)
-    _lib.call("pin_label_logprob_bwd", z.data_ptr(), _lib.TYPES[z.dtype], n, c, z.stride(0), y.data_ptr(), ctx.ignore, k,
-              top[0].data_ptr() if top else None, ctx.stats.data_ptr(), None if g_lp is None else g_lp.data_ptr(),
-              None if g_ent is None else g_ent.data_ptr(), None if g_top is None else g_top.data_ptr(), dz.data_ptr(),
-              _lib.raw_stream(z.get_device()))
-    return dz, None, None, None
-
-
-_backward_once = once_differentiable(_backward)
-
-
-class _LabelLogProbFn(torch.autograd.Function):
-    """(log_prob, entropy), and with k > 0 (top_log_prob, top_index)."""
-
-    @staticmethod
-    def forward(ctx, z, y, k, ignore):
-        ctx.set_materialize_grads(False)
-        lp, ent, stats, tlp, tidx = _forward(z, y, k, ignore, True)
-        ctx.stats, ctx.ignore = stats, ignore
-        if k == 0:
-            ctx.save_for_backward(z, y)
-            return lp, ent
-        ctx.save_for_backward(z, y, tidx)
-        ctx.mark_non_differentiable(tidx)
-        return lp, ent, tlp, tidx
-
-    @staticmethod
-    def backward(ctx, *g):
-        return _backward_once(ctx, *g) if torch.is_grad_enabled() else _backward(ctx, *g)
 
 
 def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, ignore_index: int = -100):
@@ -110,13 +68,13 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
     if y.dtype != torch.int64 or not y.is_contiguous():
         y = y.to(torch.int64).contiguous()
     with _lib.on_device(z.get_device()):
-        if torch.is_grad_enabled() and logits.requires_grad:
-            lp, ent, *top = _LabelLogProbFn.apply(z, y, k, int(ignore_index))
-        else:
-            lp, ent, _, *top = _forward(z, y, k, int(ignore_index), False)
+        grad, ignore = torch.is_grad_enabled() and logits.requires_grad, int(ignore_index)
+        lp, ent, stats, tlp, tidx = _forward(z, y, k, ignore, grad)
+        if grad and _lib.torch_fn("pin_torch_label_attach")(_lib.address("pin_label_logprob_bwd"), z, y, stats, lp, ent, tlp, tidx,
+                                                            ignore, k):
+            raise RuntimeError("label_log_probs: the gradient's inputs cannot be kept")
     if k == 0:
-        top = lp.new_empty((lp.shape[0], 0)), y.new_empty((lp.shape[0], 0))
-    tlp, tidx = top
+        tlp, tidx = lp.new_empty((lp.shape[0], 0)), y.new_empty((lp.shape[0], 0))
     if logits.dim() != 2:
         lead = labels.shape
         lp, ent, tlp, tidx = lp.view(lead), ent.view(lead), tlp.view(lead + (k,)), tidx.view(lead + (k,))

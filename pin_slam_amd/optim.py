@@ -190,7 +190,7 @@ class AdamW(torch.optim.Optimizer):
         n = len(params)
         if arena.together:   # the usual step: every parameter and every gradient as the kernel takes them
             ps, gs = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
-            if _lib.torch_gather()(params, n, arena.c_sizes.buffer_info()[0], arena.index, ps.buffer_info()[0],
+            if _lib.torch_fn("pin_torch_gather")(params, n, arena.c_sizes.buffer_info()[0], arena.index, ps.buffer_info()[0],
                                    gs.buffer_info()[0]) >= 0:
                 return [(None, params[0].dtype, ps, gs)]
         grads = [p.grad for p in params]

@@ -112,7 +112,7 @@ def test_addresses_of_many_tensors():
     import weakref
     from array import array
 
-    gather = _lib.torch_gather()
+    gather = _lib.torch_fn("pin_torch_gather")
 
     def make(kind=torch.float32, shapes=((7,), (3, 4), (), (0,))):
         out = [torch.nn.Parameter(torch.ones(s, dtype=kind)) for s in shapes]

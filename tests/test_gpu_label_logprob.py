@@ -512,5 +512,55 @@ def test_refusals(dev):
     x = z.clone().requires_grad_(True)
     r = P.label_log_probs(x, y)
     g, = torch.autograd.grad(r.log_prob.sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match="differentiate twice"):
         g.sum().backward()
+    r = P.label_log_probs(x, y)
+    r.log_prob.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        r.entropy.sum().backward()
+    r = P.label_log_probs(x, y)
+    with torch.no_grad():
+        x += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.log_prob.sum().backward()
+
+
+def test_the_node_in_torchs_graph(dev):
+    """What torch does with any operator's results: kept graphs, results changed in place, hooks, checkpoints, anomaly
+    checks, results and graphs that go without a backward pass."""
+    logits, y = make(12, 100, torch.float32, dev, ignore_some=False)
+    x = logits.detach().clone().requires_grad_(True)
+    r = P.label_log_probs(x, y, top_k=2)
+    assert r.log_prob.grad_fn is not None and r.top_index.grad_fn is None and not r.top_index.requires_grad
+    want, = torch.autograd.grad(r.log_prob.sum(), x, retain_graph=True)
+    again, = torch.autograd.grad(r.log_prob.sum(), x)
+    assert torch.equal(want, again)
+    r = P.label_log_probs(x, y, top_k=2)
+    r.log_prob.mul_(2.0)   # its own result: nothing of the node's
+    got, = torch.autograd.grad(r.log_prob.sum(), x)
+    torch.testing.assert_close(got, 2 * want, rtol=1e-6, atol=1e-6)
+    seen = []
+    r = P.label_log_probs(x, y)
+    r.log_prob.register_hook(lambda g: seen.append(g) or 3 * g)
+    got, = torch.autograd.grad(r.log_prob.sum(), x)
+    torch.testing.assert_close(got, 3 * want, rtol=1e-6, atol=1e-6)
+    assert len(seen) == 1
+    from torch.utils.checkpoint import checkpoint
+    for reentrant in (False, True):
+        out = checkpoint(lambda t: P.label_log_probs(t * 1.0, y, top_k=2).log_prob, x, use_reentrant=reentrant)
+        out.sum().backward()
+        assert torch.equal(x.grad, want)
+        x.grad = None
+    with torch.autograd.graph.save_on_cpu():
+        out = P.label_log_probs((x.t() * 1.0).t(), y, top_k=2).log_prob.sum()
+    got, = torch.autograd.grad(out, x)
+    assert torch.equal(got, want)
+    with torch.autograd.detect_anomaly(check_nan=True):
+        got, = torch.autograd.grad(P.label_log_probs(x, y).log_prob.sum(), x)
+    assert torch.equal(got, want)
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        P.label_log_probs(x, y, top_k=2)
+    assert torch.cuda.memory_allocated() == before
+    with torch.inference_mode():
+        assert not P.label_log_probs(x, y).log_prob.requires_grad
