@@ -269,7 +269,7 @@ def load():
 
 _TORCH_SIGS = {   # functions of the library that is built against torch (csrc/pin_torch.cpp)
     "pin_torch_gather": [ctypes.py_object, i64, c_void_p, i64, c_void_p, c_void_p],
-    "pin_torch_label_attach": [c_void_p] + [ctypes.py_object] * 7 + [i64, i64],
+    "pin_torch_label": [c_void_p] * 3 + [ctypes.py_object] * 2 + [i64, i64, i32],
 }
 
 
@@ -287,7 +287,7 @@ def torch_fn(name):
             raise RuntimeError(f"pin_slam_amd: {TORCH_LIB_PATH} was built for torch {built}, this is {torch.__version__}")
         for key, args in _TORCH_SIGS.items():
             getattr(lib, key).argtypes = args
-            getattr(lib, key).restype = ctypes.c_int
+            getattr(lib, key).restype = ctypes.py_object if key == "pin_torch_label" else ctypes.c_int
         _torch_lib = lib
     return getattr(_torch_lib, name)
 
@@ -352,11 +352,6 @@ def stream(device=None):
             idx = torch.cuda.current_device() if idx is None else idx
         return c_void_p(_raw_stream(idx))
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def raw_stream(index):
-    """stream() of a device by its number, as a whole number."""
-    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 _HERE_ALREADY = contextlib.nullcontext()

@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -25,9 +26,15 @@ bool as_taken(const at::Tensor& t, c10::ScalarType type, int64_t device, int64_t
 }
 
 // The gradient of label_log_probs as a node of torch's graph: the engine runs it on a thread of its own, where
-// the same in Python takes longer (forward and gradient of 64 x 20 f32: 90 us, here 60; of 16384 x 1003 f16: 105, here 73).
+// the same in Python takes longer (forward and gradient of 16384 x 1003 f16 105 us, with this node 73).
 // Outputs log_prob, entropy and, with k > 0, top_log_prob; one input, the logits [n, C].
+typedef decltype(&pin_label_logprob_workspace_bytes) LabelWorkspace;
+typedef decltype(&pin_label_logprob) LabelFwd;
 typedef decltype(&pin_label_logprob_bwd) LabelBwd;
+
+int type_of(c10::ScalarType t) {
+    return t == c10::kFloat ? PIN_TYPE_F32 : t == c10::kHalf ? PIN_TYPE_F16 : t == c10::kBFloat16 ? PIN_TYPE_BF16 : -1;
+}
 
 struct LabelNode : torch::autograd::Node {
     LabelBwd bwd = nullptr;
@@ -60,10 +67,7 @@ struct LabelNode : torch::autograd::Node {
             if (k > 0) idx = idx.contiguous();
             dz = at::empty({z.size(0), z.size(1)}, z.options());
             const auto at_f32 = [](const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; };
-            const int type = z.scalar_type() == c10::kFloat  ? PIN_TYPE_F32
-                             : z.scalar_type() == c10::kHalf ? PIN_TYPE_F16
-                                                             : PIN_TYPE_BF16;
-            const int rc = bwd(z.const_data_ptr(), type, z.size(0), z.size(1), z.stride(0), y.const_data_ptr<int64_t>(), ignore,
+            const int rc = bwd(z.const_data_ptr(), type_of(z.scalar_type()), z.size(0), z.size(1), z.stride(0), y.const_data_ptr<int64_t>(), ignore,
                                (int32_t)k, k > 0 ? idx.const_data_ptr<int64_t>() : nullptr, stats.const_data_ptr<float>(),
                                at_f32(u[0]), at_f32(u[1]), at_f32(u[2]), dz.mutable_data_ptr(),
                                (void*)c10::hip::getCurrentHIPStream(z.device().index()).stream());
@@ -76,6 +80,49 @@ struct LabelNode : torch::autograd::Node {
         return (*once)({dz});
     }
 };
+
+// Another thread may go on in Python meanwhile.
+struct NoInterpreter {
+    PyThreadState* state = PyEval_SaveThread();
+    ~NoInterpreter() { PyEval_RestoreThread(state); }
+};
+
+// What allocates and launches a forward pass: 14.5 us a call from Python, here 8.7 (1 x 32768 bf16, whose kernel takes 8.0).
+void label_forward(LabelWorkspace workspace, LabelFwd forward, LabelBwd backward, const at::Tensor& z, const at::Tensor& y,
+                   int64_t k, int64_t ignore, bool grad, at::Tensor& lp, at::Tensor& ent, at::Tensor& top_lp,
+                   at::Tensor& top_idx) {
+    const int64_t n = z.size(0), c = z.size(1);
+    const c10::DeviceGuard device(z.device());
+    const at::TensorOptions f32 = at::TensorOptions(z.device()).dtype(at::kFloat);
+    at::Tensor stats, ws;
+    lp = at::empty({n}, f32);
+    ent = at::empty({n}, f32);
+    top_lp = at::empty({n, k}, f32);
+    top_idx = at::empty({n, k}, f32.dtype(at::kLong));
+    if (grad) stats = at::empty({n, 3}, f32);
+    const int type = type_of(z.scalar_type());
+    const int64_t need = workspace(n, c, type, (int32_t)k);
+    if (need > 0) ws = at::empty({need}, f32.dtype(at::kByte));
+    const int rc = forward(z.const_data_ptr(), type, n, c, z.stride(0), y.const_data_ptr<int64_t>(), ignore, (int32_t)k,
+                           lp.mutable_data_ptr<float>(), ent.mutable_data_ptr<float>(),
+                           grad ? stats.mutable_data_ptr<float>() : nullptr, k > 0 ? top_lp.mutable_data_ptr<float>() : nullptr,
+                           k > 0 ? top_idx.mutable_data_ptr<int64_t>() : nullptr, need > 0 ? ws.mutable_data_ptr() : nullptr,
+                           (void*)c10::hip::getCurrentHIPStream(z.device().index()).stream());
+    TORCH_CHECK(rc == PIN_OK, "pin_label_logprob failed: ", rc);
+    if (!grad) return;
+    const std::shared_ptr<LabelNode> node(new LabelNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(z));
+    node->bwd = backward;
+    node->logits = torch::autograd::SavedVariable(z, false);
+    node->labels = torch::autograd::SavedVariable(y, false);
+    if (k > 0) node->top = torch::autograd::SavedVariable(top_idx, false);
+    node->stats = stats;
+    node->ignore = ignore;
+    node->k = k;
+    torch::autograd::set_history(lp, node);
+    torch::autograd::set_history(ent, node);
+    if (k > 0) torch::autograd::set_history(top_lp, node);
+}
 
 }  // namespace
 
@@ -102,37 +149,35 @@ int pin_torch_gather(PyObject* params, int64_t count, const int64_t* sizes, int6
             ps[i] = (uint64_t)(uintptr_t)p.mutable_data_ptr();
             gs[i] = (uint64_t)(uintptr_t)g.const_data_ptr();
         }
-        return type == c10::kFloat ? PIN_TYPE_F32 : type == c10::kHalf ? PIN_TYPE_F16 : type == c10::kBFloat16 ? PIN_TYPE_BF16 : -1;
+        return type_of(type);
     } catch (...) {
         return -1;
     }
 }
 
-// Makes log_prob, entropy and top_log_prob (None with k = 0) results of logits, with what pin_label_logprob left for
-// the gradient.  bwd: pin_label_logprob_bwd.  0, or -1 for what are not tensors or cannot be saved.
-int pin_torch_label_attach(void* bwd, PyObject* logits, PyObject* labels, PyObject* stats, PyObject* log_prob,
-                           PyObject* entropy, PyObject* top_log_prob, PyObject* top_index, int64_t ignore, int64_t k) {
-    for (PyObject* o : {logits, labels, stats, log_prob, entropy})
-        if (!THPVariable_Check(o)) return -1;
-    if (!bwd || (k > 0 && !(THPVariable_Check(top_log_prob) && THPVariable_Check(top_index)))) return -1;
-    try {
-        const std::shared_ptr<LabelNode> node(new LabelNode(), torch::autograd::deleteNode);
-        const at::Tensor& z = THPVariable_Unpack(logits);
-        node->set_next_edges(torch::autograd::collect_next_edges(z));
-        node->bwd = (LabelBwd)bwd;
-        node->logits = torch::autograd::SavedVariable(z, false);
-        node->labels = torch::autograd::SavedVariable(THPVariable_Unpack(labels), false);
-        if (k > 0) node->top = torch::autograd::SavedVariable(THPVariable_Unpack(top_index), false);
-        node->stats = THPVariable_Unpack(stats);
-        node->ignore = ignore;
-        node->k = k;
-        torch::autograd::set_history(THPVariable_Unpack(log_prob), node);
-        torch::autograd::set_history(THPVariable_Unpack(entropy), node);
-        if (k > 0) torch::autograd::set_history(THPVariable_Unpack(top_log_prob), node);
-        return 0;
-    } catch (...) {
-        return -1;
+// label_log_probs of checked arguments: logits [n, C] with adjacent classes, labels [n] int64 without gaps, on one device;
+// workspace, forward, backward: the kernels' library's entry points.  A new tuple (log_prob, entropy, top_log_prob,
+// top_index), results of logits where grad is set; an exception of Python's where that cannot be.
+PyObject* pin_torch_label(void* workspace, void* forward, void* backward, PyObject* logits, PyObject* labels, int64_t k,
+                          int64_t ignore, int32_t grad) {
+    if (!workspace || !forward || !backward || !THPVariable_Check(logits) || !THPVariable_Check(labels)) {
+        PyErr_SetString(PyExc_TypeError, "label_log_probs: two tensors");
+        return nullptr;
     }
+    HANDLE_TH_ERRORS
+    const at::Tensor &z = THPVariable_Unpack(logits), &y = THPVariable_Unpack(labels);
+    at::Tensor lp, ent, top_lp, top_idx;
+    {
+        const NoInterpreter released;
+        label_forward((LabelWorkspace)workspace, (LabelFwd)forward, (LabelBwd)backward, z, y, k, ignore, grad != 0, lp, ent,
+                      top_lp, top_idx);
+    }
+    PyObject* out = PyTuple_New(4);
+    if (!out) return nullptr;
+    int at = 0;
+    for (const at::Tensor* t : {&lp, &ent, &top_lp, &top_idx}) PyTuple_SET_ITEM(out, at++, THPVariable_Wrap(*t));
+    return out;
+    END_HANDLE_TH_ERRORS
 }
 
 }  // extern "C"

@@ -3,8 +3,8 @@
 The loss beside the classification heads (model/decoder.py:120: log_softmax and argmax over
 the classes): one pass over the logits gives what a training loss, a confidence and a list of
 alternatives need, and the gradient recomputes the probabilities from the logits, so nothing of
-the logits' size is kept between the two (pin_label_logprob, pin_label_logprob_bwd).  The
-gradient's node in torch's graph is native (csrc/pin_torch.cpp).
+the logits' size is kept between the two (pin_label_logprob, pin_label_logprob_bwd).  Both,
+and the node in torch's graph, are called natively (csrc/pin_torch.cpp): small calls are the host's.
 """
 from collections import namedtuple
 
@@ -13,25 +13,6 @@ import torch
 from . import _lib
 
 LabelLogProbs = namedtuple("LabelLogProbs", ["log_prob", "entropy", "top_log_prob", "top_index"])
-
-
-def _forward(z, y, k, ignore, want_stats):
-    """log_prob [n], entropy [n], row statistics [n, 3] or None, top_log_prob and top_index [n, k] or None, of the
-    rows z [n, C]."""
-    n, c = z.shape
-    dev = z.device
-    lp = torch.empty((n,), dtype=torch.float32, device=dev)
-    ent = torch.empty((n,), dtype=torch.float32, device=dev)
-    stats = torch.empty((n, 3), dtype=torch.float32, device=dev) if want_stats else None
-    tlp = torch.empty((n, k), dtype=torch.float32, device=dev) if k else None
-    tidx = torch.empty((n, k), dtype=torch.int64, device=dev) if k else None
-    dt = _lib.TYPES[z.dtype]
-    need = _lib.fn("pin_label_logprob_workspace_bytes")(n, c, dt, k)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-    _lib.call("pin_label_logprob", z.data_ptr(), dt, n, c, z.stride(0), y.data_ptr(), ignore, k, lp.data_ptr(),
-              ent.data_ptr(), stats.data_ptr() if want_stats else None, tlp.data_ptr() if k else None,
-              tidx.data_ptr() if k else None, None if ws is None else ws.data_ptr(), _lib.raw_stream(z.get_device()))
-    return lp, ent, stats, tlp, tidx
 
 
 def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, ignore_index: int = -100):
@@ -67,14 +48,10 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
         z = z.contiguous()
     if y.dtype != torch.int64 or not y.is_contiguous():
         y = y.to(torch.int64).contiguous()
-    with _lib.on_device(z.get_device()):
-        grad, ignore = torch.is_grad_enabled() and logits.requires_grad, int(ignore_index)
-        lp, ent, stats, tlp, tidx = _forward(z, y, k, ignore, grad)
-        if grad and _lib.torch_fn("pin_torch_label_attach")(_lib.address("pin_label_logprob_bwd"), z, y, stats, lp, ent, tlp, tidx,
-                                                            ignore, k):
-            raise RuntimeError("label_log_probs: the gradient's inputs cannot be kept")
-    if k == 0:
-        tlp, tidx = lp.new_empty((lp.shape[0], 0)), y.new_empty((lp.shape[0], 0))
+    lp, ent, tlp, tidx = _lib.torch_fn("pin_torch_label")(
+        _lib.address("pin_label_logprob_workspace_bytes"), _lib.address("pin_label_logprob"),
+        _lib.address("pin_label_logprob_bwd"), z, y, k, int(ignore_index),
+        1 if logits.requires_grad and torch.is_grad_enabled() else 0)
     if logits.dim() != 2:
         lead = labels.shape
         lp, ent, tlp, tidx = lp.view(lead), ent.view(lead), tlp.view(lead + (k,)), tidx.view(lead + (k,))

@@ -107,6 +107,12 @@ def test_argument_errors_before_any_device_work():
     assert lib.pin_adamw_moments(ok, ok, ok, 0, None, None, None) == 0
 
 
+def test_what_is_no_tensor_is_refused():
+    fns = [_lib.address(n) for n in ("pin_label_logprob_workspace_bytes", "pin_label_logprob", "pin_label_logprob_bwd")]
+    with pytest.raises(TypeError, match="two tensors"):
+        _lib.torch_fn("pin_torch_label")(*fns, 3, torch.zeros(2, dtype=torch.int64), 0, -100, 1)
+
+
 def test_addresses_of_many_tensors():
     """pin_torch_gather: addresses of what is as the kernel takes it, refusal of anything else (host tensors, device -1)."""
     import weakref
