@@ -1,9 +1,10 @@
-// pin_torch.cpp -- what is asked of torch's own objects, many at a time, in a library of its own
+// pin_torch.cpp -- what is done with torch's own objects, host code in a library of its own
 // (libpin_slam_torch.so): the kernels' library knows no torch.
 //
-// An optimiser step needs two addresses and ten properties per parameter.  Asked from Python they
-// cost 0.43 us per parameter, which for a few hundred small ones is more than the step's kernels
-// (331 parameters, 13M elements: 77 us); here 0.01.
+// pin_torch_gather: an optimiser step needs two addresses and ten properties per parameter.  Asked
+// from Python they cost 0.43 us per parameter, which for a few hundred small ones is more than the
+// step's kernels (331 parameters, 13M elements: 77 us); here 0.01.
+// pin_torch_label: label_log_probs' outputs, launch and node in torch's graph, in one call.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
