@@ -64,12 +64,12 @@ struct LabelNode : torch::autograd::Node {
             y = y.contiguous();
             at::Tensor u[3];
             for (size_t i = 0; i < grads.size() && i < 3; ++i)
-                if (grads[i].defined()) u[i] = grads[i].to(at::kFloat).contiguous();
+                if (grads[i].defined()) u[i] = grads[i].to(at::kFloat).resolve_neg().contiguous();
             if (k > 0) idx = idx.contiguous();
             dz = at::empty({z.size(0), z.size(1)}, z.options());
             const auto at_f32 = [](const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; };
-            const int rc = bwd(z.const_data_ptr(), type_of(z.scalar_type()), z.size(0), z.size(1), z.stride(0), y.const_data_ptr<int64_t>(), ignore,
-                               (int32_t)k, k > 0 ? idx.const_data_ptr<int64_t>() : nullptr, stats.const_data_ptr<float>(),
+            const int rc = bwd(z.const_data_ptr(), type_of(z.scalar_type()), z.size(0), z.size(1), z.stride(0),
+                               y.const_data_ptr<int64_t>(), ignore, (int32_t)k, k > 0 ? idx.const_data_ptr<int64_t>() : nullptr, stats.const_data_ptr<float>(),
                                at_f32(u[0]), at_f32(u[1]), at_f32(u[2]), dz.mutable_data_ptr(),
                                (void*)c10::hip::getCurrentHIPStream(z.device().index()).stream());
             TORCH_CHECK(rc == PIN_OK, "pin_label_logprob_bwd failed: ", rc);
@@ -92,6 +92,7 @@ struct NoInterpreter {
 void label_forward(LabelWorkspace workspace, LabelFwd forward, LabelBwd backward, const at::Tensor& z, const at::Tensor& y,
                    int64_t k, int64_t ignore, bool grad, at::Tensor& lp, at::Tensor& ent, at::Tensor& top_lp,
                    at::Tensor& top_idx) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!z._fw_grad(0).defined(), "label_log_probs: forward-mode differentiation is not implemented");
     const int64_t n = z.size(0), c = z.size(1);
     const c10::DeviceGuard device(z.device());
     const at::TensorOptions f32 = at::TensorOptions(z.device()).dtype(at::kFloat);

@@ -46,6 +46,8 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
         z, y = logits.reshape(labels.numel(), c), labels.reshape(-1)
     if c > 1 and z.stride(1) != 1:
         z = z.contiguous()
+    if z.is_neg():
+        z = z.resolve_neg()
     if y.dtype != torch.int64 or not y.is_contiguous():
         y = y.to(torch.int64).contiguous()
     lp, ent, tlp, tidx = _lib.torch_fn("pin_torch_label")(

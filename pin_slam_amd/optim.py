@@ -181,7 +181,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: a parameter was reshaped or moved after its first step")
         if g.dtype != p.dtype or g.device != arena.device or p.dtype not in _lib.TYPES or g.numel() != arena.sizes[i]:
             raise RuntimeError(f"AdamW: a {p.dtype} parameter on {p.device} has a {g.dtype} gradient on {g.device}")
-        return g if g.is_contiguous() else g.contiguous()
+        if p.is_neg():
+            raise RuntimeError("AdamW: a parameter is a negated view")
+        return g.resolve_neg().contiguous()
 
     def _gather(self, arena, group):
         """What has a gradient, checked: launches of (indexes or None for all, their type, addresses of the parameters and

@@ -522,6 +522,15 @@ def test_gradients_in_other_layouts(dev):
     assert torch.equal(p, q)
 
 
+def test_a_negated_view_as_gradient(dev):
+    a, b = tensors([1000], torch.float32, dev), tensors([1000], torch.float32, dev)
+    set_grads(a, 3)
+    b[0].grad = torch._neg_view(-a[0].grad)
+    for p in (a, b):
+        P.AdamW(p, **HYPER).step()
+    assert b[0].grad.is_neg() and torch.equal(a[0], b[0])
+
+
 def test_more_elements_than_32_bits_count(dev):
     """2^31 + 300 elements with moments in 8 bits: the first and last blocks as a small tensor's at the same places."""
     n = (1 << 31) + 300

@@ -525,6 +525,22 @@ def test_refusals(dev):
         r.log_prob.sum().backward()
 
 
+def test_views_that_negate_and_forward_mode(dev):
+    logits, y = make(9, 100, torch.float32, dev, ignore_some=False)
+    x = logits.detach().clone().requires_grad_(True)
+    r = P.label_log_probs(x, y, top_k=2)
+    up = torch.randn((9,), generator=torch.Generator().manual_seed(1)).to(dev)
+    want, = torch.autograd.grad(r.log_prob, x, up)
+    n = torch._neg_view(-x)
+    got = P.label_log_probs(n, y, top_k=2)
+    assert n.is_neg() and all(torch.equal(a, b) for a, b in zip(got, r))
+    g, = torch.autograd.grad(got.log_prob, x, torch._neg_view(-up))
+    assert torch.equal(g, want)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        P.label_log_probs(fwd.make_dual(logits, torch.ones_like(logits)), y)
+
+
 def test_the_node_in_torchs_graph(dev):
     """What torch does with any operator's results: kept graphs, results changed in place, hooks, checkpoints, anomaly
     checks, results and graphs that go without a backward pass."""
