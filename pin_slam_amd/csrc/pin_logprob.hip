@@ -12,9 +12,11 @@
 // for the classes.  Sums and statistics are f32 whatever the logits' type.
 //
 // The exponentials are taken to base 2: x_j = z_j L - fl(m L), L = log2 e, in one fma.  fl(m L)
-// shifts every x_j of a row alike, and every result is a difference of such, so its rounding
-// cancels.  Where m L leaves the range of f32 (rows masked by the type's lowest value throughout)
-// x_j = (z_j - m) L.
+// shifts every x_j of a row alike, by its rounding (up to 2^-25 |m L|), and every result is a
+// difference of such.  The shift has to stay small, as 2^x is taken before the difference: at
+// |m| = 3e9 it is 2^7, and the sum infinite or 0.  So beyond |m| = 2^20, where it is 2^-4, x_j =
+// (z_j - m) L, without a shift: rows masked throughout by a large finite value, and the parts of
+// rows that are, in whatever a maximum is taken of.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -26,6 +28,7 @@ namespace {
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kL = 1.44269504f, kLn2 = 0.693147182f;
 constexpr float kFloor = -1000.f;            // 2^x is 0 well above
+constexpr float kNear = 0x1p20f;             // largest size of a maximum m whose fl(m L) is taken (see above)
 // most classes of the kernels of one thread per row (300000 x 64 f32 with 3 alternatives: 38 us, sixteen lanes 51)
 constexpr int kSmall = 64;
 constexpr int kSplits = 64;                  // most parts of a row
@@ -219,14 +222,14 @@ __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_el
 
 struct Row {
     float m, ls;   // maximum (+inf: the row has a NaN or +inf; -inf: nothing in it), log2 of the sum
-    float ml;      // fl(m L), where that is finite
-    bool far;      // it is not
-    __device__ __forceinline__ explicit Row(float max) : m(max), ls(0.f), ml(max * kL), far(!(fabsf(max) <= 0x1p127f)) {}
+    float ml;      // fl(m L), what is subtracted where m is not far
+    bool far;      // (z - m) L then
+    __device__ __forceinline__ explicit Row(float max) : m(max), ls(0.f), ml(max * kL), far(!(fabsf(max) <= kNear)) {}
     __device__ __forceinline__ bool bad() const { return m == kInf; }
     __device__ __forceinline__ bool dead() const { return m == -kInf; }
     __device__ __forceinline__ float x(float z) const { return far ? (z - m) * kL : fmaf(z, kL, -ml); }
     __device__ __forceinline__ float log_prob(float z) const {
-        const float v = (x(z) - ls) * kLn2;
+        const float v = far ? fmaf(-ls, kLn2, z - m) : (x(z) - ls) * kLn2;
         // where only z L is out of range: log s is nothing beside z - m
         return bad() ? NAN : dead() ? -kInf : v == -kInf ? z - m : v;
     }
@@ -669,7 +672,10 @@ __device__ __forceinline__ Row join_sums(const float4* __restrict__ sums, const 
     const int64_t y = labels[row];
     const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
     Row r(wave_max(p.x));
-    const float x = fmaxf(r.far ? (p.x - r.m) * kL : p.x * kL - r.ml, kFloor);
+    // to the row's form from the one in which the part was summed: the row's own shift less the part's
+    const Row q(p.x);
+    const float x = fmaxf(r.far ? (q.far ? (p.x - r.m) * kL : -fmaf(r.m, kL, -q.ml)) : q.far ? fmaf(p.x, kL, -r.ml) : q.ml - r.ml,
+                          kFloor);
     const float f = __builtin_amdgcn_exp2f(x);
     const float s = wave_sum(f * p.y), t = wave_sum(f * fmaf(p.y, x, p.z));
     r.ls = r.dead() ? 0.f : __builtin_amdgcn_logf(s);
@@ -843,7 +849,9 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
     if (tid == 0) s_m.clear();
     const int64_t y = labels[row];
     const float zy = y >= 0 && y < classes ? T::one(zr + y) : 0.f;
-    constexpr float kLow = -0x1p126f;
+    // m L is taken of maxima down to -kNear only: of a thread whose classes all lie below nothing reaches the sums,
+    // unless the whole row does (or lies above kNear), which is summed again
+    constexpr float kLow = -kNear;
     float m = -kInf, ml = kLow * kL, s = 0.f, t = 0.f;
 #pragma unroll 1
     for (int p = 0; p < parts; ++p) {
@@ -883,13 +891,17 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
     if (lane == 0) s_sum[wave].z = wm;
     __syncthreads();
     Row r(fmaxf(fmaxf(s_sum[0].z, s_sum[1].z), fmaxf(s_sum[2].z, s_sum[3].z)));
-    if (fabsf(r.m) > 0x1p126f && !r.bad() && !r.dead()) {   // no thread's maximum was one to take 2^x to
+    if (r.far && !r.bad() && !r.dead()) {
         s = t = 0.f;
-        r.far = true;
-        for (int j = tid; j < classes; j += 256) {
-            const float x = fmaxf(r.x(T::one(zr + j)), kFloor), e = __builtin_amdgcn_exp2f(x);
-            s += e;
-            t = fmaf(e, x, t);
+#pragma unroll 1
+        for (int p = 0; p < parts; ++p) {
+            const int u0 = p * kPart, u1 = u0 + kPart < z.count ? u0 + kPart : z.count;
+            uint4 q[NCH];
+            load_part<T, 4, NCH>(z, u0, u1, q);
+            float ps, pt;
+            part_sums<T, 4, NCH>(r, q, u1 - u0, ps, pt);
+            s += ps;
+            t += pt;
         }
     } else {
         const float x = fmaxf(ml - r.ml, kFloor), f = __builtin_amdgcn_exp2f(x);
@@ -1089,7 +1101,8 @@ k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int classes,
     const float pz = given ? T::one(z + pj) : 0.f;
     float more = top ? u.top[row * k + g] : 0.f;
     const RowGrad d(stats, u, on ? row : 0, y, ignore, classes, u.top ? sum_of<LANES>(more) : 0.f);
-    const bool plain = !d.r.far && !d.r.bad() && !d.r.dead();
+    const bool plain = !d.r.bad() && !d.r.dead(), some_far = __any(d.r.far);
+    const float off = d.r.far ? 0.f : d.r.ml, from = d.r.far ? d.r.m : 0.f;   // x = (z - from) L - off
     if (on) {
         for (int v0 = u0 + lane; v0 < u1; v0 += LANES * B) {
             uint4 q[B];
@@ -1106,9 +1119,13 @@ k_label_bwd(const typename T::type* __restrict__ logits, int64_t n, int classes,
                 if (w.whole(v) && plain) {
                     float f[V];
                     T::unpack(q[c], f);
+                    if (some_far) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) f[i] -= from;
+                    }
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float x = fmaxf(fmaf(f[i], kL, -d.r.ml) - d.r.ls, kFloor);
+                        const float x = fmaxf(fmaf(f[i], kL, -off) - d.r.ls, kFloor);
                         f[i] = -__builtin_amdgcn_exp2f(x) * fmaf(d.gh, x + d.h, d.g);
                     }
                     *(uint4*)(o + j) = T::pack(f);

@@ -265,6 +265,62 @@ def test_masks_ties_and_values_of_many_rows(dev, c, times, kind):
         check(z.repeat(times, 1).to(dev), y.repeat(times).to(dev), k)
 
 
+FILLS = [1e6, 5e7, 5e9, 1e10, 1e12, 1e20, 1e30]
+
+
+def finite_mask_rows(c, kind, seed=0):
+    """Rows in which a large finite value stands in all classes, in most, or in a range beside ordinary ones, below
+    them (a mask that programs write in -inf's place) or above."""
+    g = torch.Generator().manual_seed(seed + 7 * c)
+    base = torch.randn((c,), generator=g)
+    rows, labels = [], []
+    off = torch.rand((c,), generator=g) < 0.9
+    off[c // 3] = False
+    part = torch.zeros((c,), dtype=torch.bool)
+    part[c // 8:c // 8 + (c + 1) // 2] = True
+    for i, size in enumerate(FILLS):
+        for fill in (-size, size):
+            rows.append(torch.full((c,), fill))
+            labels.append(IGNORE if i % 2 else c // 2)
+            if fill < 0 or i in (0, 3, 6):
+                rows += [torch.where(off, fill, base), torch.where(part, fill, base)]
+                labels += [c // 3, 0 if i % 2 else c // 8]
+    spread = base * 1e10
+    rows += [spread, spread - 1e12, torch.where(part, -1e30, -1e10 + 1e4 * base), torch.where(part, 1e6, 1e6 + 1e5 * base),
+             torch.where(part, -1e12, (1 << 20) + base)]
+    labels += [0, c - 1, c // 3, 0, c // 3]
+    return torch.stack(rows).to(kind), torch.tensor(labels)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("c", [1, 2, 20, 64, 100, 700, 2500, 9001, 40000, 131073])
+def test_large_finite_masks(dev, c, kind):
+    """Every layout of few rows: no result and no gradient is lost to the size of a mask."""
+    z, y = finite_mask_rows(c, TYPES[kind])
+    for k in sorted({0, min(c, 3), min(c, 32)}):
+        check(z.to(dev), y.to(dev), k)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("c,times", [(100, 120), (700, 120), (20003, 8)])
+def test_large_finite_masks_of_many_rows(dev, c, times, kind):
+    z, y = finite_mask_rows(c, TYPES[kind])
+    for k in (0, 2, 32):
+        check(z.repeat(times, 1).to(dev), y.repeat(times).to(dev), k)
+
+
+def test_an_ignored_row_masked_by_a_finite_value_passes_no_gradient(dev):
+    """What a padded row leaves in the gradient of the layer before it: nothing."""
+    for c in (20, 700, 9001, 131073):
+        for fill in (-5e9, -1e10, -1e12, -1e30):
+            z = torch.randn((3, c), generator=torch.Generator().manual_seed(c)).to(dev)
+            z[1] = fill
+            x = z.requires_grad_(True)
+            r = P.label_log_probs(x, torch.tensor([0, IGNORE, c - 1], device=dev))
+            dz, = torch.autograd.grad(r.log_prob.sum(), x)
+            assert not bool(dz[1].any()) and bool(torch.isfinite(dz).all())
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("times", [1, 33])
 def test_large_values_in_one_place(dev, kind, times):
