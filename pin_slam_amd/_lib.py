@@ -269,6 +269,7 @@ def load():
 
 _TORCH_SIGS = {   # functions of the library that is built against torch (csrc/pin_torch.cpp)
     "pin_torch_gather": [ctypes.py_object, i64, c_void_p, i64, c_void_p, c_void_p],
+    "pin_torch_touched": [ctypes.py_object],
     "pin_torch_label": [c_void_p] * 3 + [ctypes.py_object] * 2 + [i64, i64, i32],
 }
 

@@ -4,6 +4,7 @@
 // pin_torch_gather: an optimiser step needs two addresses and ten properties per parameter.  Asked
 // from Python they cost 0.43 us per parameter, which for a few hundred small ones is more than the
 // step's kernels (331 parameters, 13M elements: 77 us); here 0.01.
+// pin_torch_touched: what was written through an address is marked as modified, as torch's own operators do.
 // pin_torch_label: label_log_probs' outputs, launch and node in torch's graph, in one call.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -152,6 +153,24 @@ int pin_torch_gather(PyObject* params, int64_t count, const int64_t* sizes, int6
             gs[i] = (uint64_t)(uintptr_t)g.const_data_ptr();
         }
         return type_of(type);
+    } catch (...) {
+        return -1;
+    }
+}
+
+// tensors: a list of tensors that a kernel writes through their addresses.  Their versions are raised, on which
+// torch's check of saved tensors and this package's derived views go (tensors made in inference mode have none).
+// 0, or -1 where one of them is no tensor.  Called with the interpreter's lock; no exception leaves it.
+int pin_torch_touched(PyObject* tensors) {
+    if (!PyList_CheckExact(tensors)) return -1;
+    try {
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
+            PyObject* o = PyList_GET_ITEM(tensors, i);
+            if (!THPVariable_Check(o)) return -1;
+            const at::Tensor& t = THPVariable_Unpack(o);
+            if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
+        return 0;
     } catch (...) {
         return -1;
     }

@@ -55,6 +55,7 @@ class _Arena:
         self.step_dev = torch.zeros((1,), dtype=torch.int64, device=dev) if capturable else None
         self.scalars = torch.zeros((_lib.ADAMW_SCALARS_BYTES,), dtype=torch.uint8, device=dev) if capturable else None
         self.start(params)
+        self.written = self.arrays()      # by every step
 
     def arrays(self):
         return [x for x in (self.m, self.v, self.exps, self.master, self.step_dev) if x is not None]
@@ -96,7 +97,9 @@ class AdamW(torch.optim.Optimizer):
 
     capturable: step() may be captured into a graph after one eager step; a group's parameters then
     all have gradients and count steps together, and lr may be a float32 tensor on the device that
-    replays read (a number is taken as it was when captured).
+    replays read (a number is taken as it was when captured).  A replay cannot mark the parameters as
+    modified: what is derived from them (a map's or decoder's views among it) goes by
+    torch.autograd.graph.increment_version(parameters) after it.
 
     The state is made at the first step (or by load_state_dict); parameters are neither added to a
     group, reshaped nor moved to another device afterwards."""
@@ -235,6 +238,12 @@ class AdamW(torch.optim.Optimizer):
     def _salt(self, gi):
         return (self.seed * _SALT_SEED + gi * _SALT_GROUP) & 0xFFFFFFFF
 
+    @staticmethod
+    def _touched(tensors):
+        """Marked as modified in place: a step writes through addresses."""
+        if _lib.torch_fn("pin_torch_touched")(tensors) != 0:
+            raise RuntimeError("AdamW: a parameter is not a tensor")
+
     def _step_group(self, gi, group, arena, todo):
         lr, (b1, b2) = group["lr"], group["betas"]
         stream = _lib.stream(arena.device)
@@ -246,8 +255,10 @@ class AdamW(torch.optim.Optimizer):
                       _lib.ptr(arena.scalars), stream)
         for idx, dtype, ps, gs in todo:
             if idx is None:
+                self._touched(group["params"] + arena.written)
                 n, sizes, offsets = len(ps), arena.c_sizes, arena.c_offsets
             else:
+                self._touched([group["params"][i] for i in idx] + arena.written)
                 n = len(idx)
                 sizes, offsets = (array("q", [x[i] for i in idx]) for x in (arena.sizes, arena.offsets))
             t = arena.steps[0 if idx is None else idx[0]] + (0 if self.capturable else 1)

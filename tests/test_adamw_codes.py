@@ -170,3 +170,20 @@ def test_addresses_of_many_tensors():
     gone = weakref.ref(p)   # no reference is kept
     del p
     assert gone() is None
+
+
+def test_versions_of_what_is_written():
+    """pin_torch_touched raises the versions that torch's check of saved tensors goes by (of tensors that have one)."""
+    touched = _lib.torch_fn("pin_torch_touched")
+    p = torch.nn.Parameter(torch.ones(4))
+    flat = torch.zeros(8)
+    view = flat[2:4]
+    with torch.inference_mode():
+        free = torch.ones(3)
+    out = (p * p).sum()
+    before = p._version
+    assert touched([p, flat, free]) == 0
+    assert p._version == before + 1 and flat._version == view._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+    assert touched([]) == 0 and touched([p, 3]) == -1 and touched((p,)) == -1

@@ -632,6 +632,90 @@ def test_a_captured_training_step(dev, bits):
                                                      [*want, q, q.grad, *ref.moments(), ref.master()]))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_query_after_a_step_sees_it(dev, bits):
+    """A map's queries read views of its features and decoder that are kept until those are modified: after a step they
+    are made anew, as a decoder and a map with the same values and no views give."""
+    from pin_slam_amd.synthetic import surface_map, surface_pool
+    nm, dec, pts = surface_map(200, device=dev, buffer_size=1 << 22, query_backend="grid")
+    q = surface_pool(pts, 5000, seed=3, device=dev)[0]
+    ask = lambda d: P.query_sdf(nm, d, q, query_locally=True, want_grad=True)[:2]   # noqa: E731
+    feats = nm.local_geo_features
+    for params in ([*dec.parameters()], [feats], [feats, *dec.parameters()]):
+        for p in params:
+            p.grad = torch.full_like(p, 0.1)
+        if len(params) > 1:
+            params[-1].grad = torch._neg_view(-params[-1].grad)   # one that is copied first
+        opt = P.AdamW(params, lr=0.05, state_bits=bits)
+        for _ in range(2):
+            before = ask(dec)
+            opt.step()
+            after = ask(dec)
+            nm._cache = {}
+            copied = P.Decoder(nm.config, 64, 1, 1)
+            copied.load_state_dict(dec.state_dict())
+            fresh = ask(copied)
+            assert not torch.equal(before[0], after[0])
+            assert all(torch.equal(a, b) for a, b in zip(after, fresh))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_between_forward_and_backward_is_seen(dev, bits):
+    """A graph that saved a parameter refuses to go back through it after a step, as with torch's optimisers."""
+    for way in ("fast", "some", "copied"):
+        params = tensors([500, 20], torch.float32, dev)
+        set_grads(params, 1)
+        if way == "copied":
+            params[0].grad = torch._neg_view(-params[0].grad)
+        opt = P.AdamW(params, state_bits=bits, **HYPER)
+        if way == "some":
+            opt.step()
+            params[1].grad = None
+        out = [(p * p).sum() for p in params]
+        versions = [p._version for p in params]
+        opt.step()
+        assert params[0]._version > versions[0] and (params[1]._version > versions[1]) == (way != "some")
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out[0].backward()
+        if way == "some":
+            out[1].backward()
+        st = opt.state[params[0]]
+        before = {k: t._version for k, t in st.items()}
+        opt.step()
+        assert all(t._version > before[k] for k, t in st.items())
+    logits = torch.nn.Parameter(torch.randn((30, 20), device=dev))
+    r = P.label_log_probs(logits, torch.zeros((30,), dtype=torch.int64, device=dev))
+    logits.grad = torch.ones_like(logits)
+    P.AdamW([logits], state_bits=bits, **HYPER).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.log_prob.sum().backward()
+
+
+def test_queries_between_replays(dev):
+    """A replayed step marks nothing: increment_version does, as documented."""
+    from pin_slam_amd.synthetic import surface_map, surface_pool
+    nm, dec, pts = surface_map(200, device=dev, buffer_size=1 << 22, query_backend="grid")
+    q = surface_pool(pts, 3000, seed=3, device=dev)[0]
+    params = [nm.local_geo_features, *dec.parameters()]
+    for p in params:
+        p.grad = torch.full_like(p, 0.1)
+    opt = P.AdamW(params, lr=0.05, capturable=True)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        torch.autograd.graph.increment_version(params)
+        after = P.query_sdf(nm, dec, q, query_locally=True, want_grad=True)[:2]
+        nm._cache = {}
+        copied = P.Decoder(nm.config, 64, 1, 1)
+        copied.load_state_dict(dec.state_dict())
+        fresh = P.query_sdf(nm, copied, q, query_locally=True, want_grad=True)[:2]
+        assert all(torch.equal(a, b) for a, b in zip(after, fresh))
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
