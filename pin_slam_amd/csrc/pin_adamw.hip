@@ -234,9 +234,12 @@ __device__ __forceinline__ uint32_t encode_v(double x, int e, uint32_t dither) {
 }
 
 // One wave per block of 256 elements, four per lane.  The parameter's step is taken in f32 from the new
-// averages before they are coded, numerator and denominator over the power of two of the block's largest
-// square root: they are normal numbers at any size of the gradients, which the hardware's square root and
-// reciprocal (one unit in the last place each) need.
+// averages before they are coded, numerator and denominator over a power of two: that of the block's largest
+// square root or of eps, whichever is larger, so that the denominator is at most a few units whatever the
+// size of the gradients and however far the second moment has decayed.  What the hardware's square root and
+// reciprocal (one unit in the last place each) need is normal numbers.  Elements for which that does not give
+// them (a second moment far below its block's largest with hardly any eps beside it, a first moment that is
+// beyond f32 over the power of two) take the step in 64 bits.
 template <class T, bool MASTER>
 __global__ void __launch_bounds__(kBlock)
 k_adamw8(AdamwTable t, uint32_t* __restrict__ m_, uint32_t* __restrict__ v_, short2* __restrict__ e_,
@@ -267,14 +270,30 @@ k_adamw8(AdamwTable t, uint32_t* __restrict__ m_, uint32_t* __restrict__ v_, sho
         m[j] = (double)cm[j] * sm + d * a.c1;
         v[j] = (double)decode_v((uv >> 8 * j) & 0xFF) * sv + d * d * a.c2;
     }
-    const int em = block_exponent(m), ev = block_exponent(v), half = ev >> 1;
+    const int em = block_exponent(m), ev = block_exponent(v), ee = ((__float_as_int(eps) >> 23) & 0xFF) - 127;
+    const int half = ev >> 1 > ee ? ev >> 1 : ee;   // (ee of 0 is -127)
     const double down = pow2(-half), down2 = pow2(-2 * half);
     const float inv = 1.f / a.bc2_sqrt, eps_down = (float)((double)eps * down);
+    float d[4], vs[4], ms[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        vs[j] = (float)(v[j] * down2);
+        ms[j] = (float)(m[j] * down);
+        d[j] = ms[j] * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(vs[j]), inv, eps_down));
+    }
+    // Beside this much of eps, what f32 cannot hold of a second moment (2^-126 and less) adds nothing.
+    if (eps_down < inv * 0x1p-36f || em - half > 125) {   // the same for the wave
+        // a first moment of zero asks for no more than a denominator that is not
+        const float still = eps_down >= 0x1p-100f ? 0.f : 0x1p-100f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (!(vs[j] >= (m[j] == 0.0 ? still : 0x1p-100f) && fabsf(ms[j]) <= 0x1p126f))
+                d[j] = (float)(m[j] / (sqrt(v[j]) * (double)inv + (double)eps));
+    }
     uint32_t om = 0, ov = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float den = fmaf(__builtin_amdgcn_sqrtf((float)(v[j] * down2)), inv, eps_down);
-        p[j] = p[j] * a.decay - a.step_size * ((float)(m[j] * down) * __builtin_amdgcn_rcpf(den));
+        p[j] = p[j] * a.decay - a.step_size * d[j];
         const uint32_t h = mix32(a.key + ((uint32_t)s + j) * kMix3);
         om |= encode_m(m[j], em, h & 0x1FFFF) << 8 * j;
         ov |= encode_v(v[j], ev, h >> 15) << 8 * j;

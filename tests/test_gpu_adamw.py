@@ -250,6 +250,57 @@ def test_zero_gradients(dev, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("kind,master", [("f32", False), ("bf16", True)])
+@pytest.mark.parametrize("betas,eps,steps", [((0.9, 0.0), 1e-8, 3), ((0.9, 0.0), 1e-15, 3), ((0.9, 0.5), 1e-8, 420),
+                                             ((0.99, 0.9), 1e-8, 2300), ((0.9, 0.5), 1e-15, 420)])
+def test_gradients_that_stop(dev, bits, kind, master, betas, eps, steps):
+    """Steps without a gradient after one with: the second moment goes faster than the first, to zero at once where
+    beta2 is 0, and what is left of the step goes by eps."""
+    params = tensors([1000, 300], TYPES[kind], dev)
+    opt = P.AdamW(params, state_bits=bits, master_weights=master, lr=1e-12, betas=betas, eps=eps, weight_decay=0.1)
+    set_grads(params, 1)
+    check_step(opt, 1)
+    for p in params:
+        p.grad.zero_()
+    t = 1
+    while t < steps:
+        at = min(steps, t + 1 if t < 3 else 2 * t)
+        for _ in range(at - t - 1):
+            opt.step()
+        t = at
+        check_step(opt, t)
+    assert all(bool(torch.isfinite(p).all()) for p in params)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30, 1e-15, 1.0])
+@pytest.mark.parametrize("small", [1e-9, 1e-20, 1e-25, 1e-30])
+def test_tiny_gradients_beside_large_ones(dev, eps, small):
+    """One block, gradients far apart: with 8 bits the averages are formed in 64 bits, and so is the step where 32 would
+    not hold what it is made of."""
+    p = tensors([700], torch.float32, dev)[0]
+    opt = P.AdamW([p], state_bits=8, lr=0.01, betas=(0.9, 0.99), eps=eps)
+    for t in (1, 2):
+        p.grad = torch.full_like(p, small) * (1 + torch.arange(700, device=dev) % 7)
+        p.grad[17], p.grad[300], p.grad[301] = 1e6, 1e12, -1e-3
+        check_step(opt, t)
+
+
+def test_untouched_elements_without_eps(dev):
+    """eps 0 and moments of zero: 0/0, not a number, as the formula has it; elements with a gradient step as ever."""
+    for bits in (32, 8):
+        p = tensors([600], torch.float32, dev)[0]
+        opt = P.AdamW([p], state_bits=bits, lr=0.01, betas=(0.9, 0.99), eps=0.0)
+        p.grad = torch.ones_like(p)
+        p.grad[::3] = 0
+        p0 = p.detach().clone()
+        opt.step()
+        zero = torch.zeros_like(p, dtype=torch.bool)
+        zero[::3] = True
+        assert torch.equal(torch.isnan(p), zero)
+        torch.testing.assert_close(p.detach()[~zero], p0[~zero] - 0.01, rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_not_a_number_stays_in_its_place(dev, bits):
     p = tensors([1500], torch.float32, dev)[0]
     opt = P.AdamW([p], state_bits=bits, **HYPER)
