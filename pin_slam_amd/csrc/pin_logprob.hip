@@ -1219,6 +1219,8 @@ struct Plan {
 constexpr int64_t kManyRows = 4096;
 constexpr int64_t kFull = 1024;    // workgroups that fill the chip
 constexpr int64_t kBatch = 1 << 23;  // rows of one launch
+constexpr int64_t kGrid = (1 << 24) - 1;  // workgroups of 256 threads of one launch: it has fewer than 2^32 threads
+static_assert(kBatch <= kGrid && kGrid / kSplits >= kFull, "a batch of split rows is many");
 // ... when each has a workgroup to itself, or its rows are short: 256 x 50021 bf16 with 20 alternatives 16.8 us
 // (in parts, joined, 21.9), 1 x 32768 with 5 8.0 (9.0), but 1 x 131072 with 20 19.6 (12.5).
 constexpr int64_t kRows = 256;
@@ -1257,6 +1259,9 @@ Plan plan_rows(int64_t n, int64_t classes, int v, int k) {
     p.part = (int)((vecs + p.splits - 1) / p.splits);
     return p;
 }
+
+// Rows of one launch, and so rows whose parts lie in the workspace at a time.
+inline int64_t batch_of(const Plan& p) { return p.splits > 1 ? kGrid / p.splits : kBatch; }
 
 inline uint32_t magic_of(int64_t classes) { return (uint32_t)((1 << 20) / classes + 1); }
 
@@ -1311,7 +1316,6 @@ int forward_rows(const Call& a, const Plan& p) {
         else go(k_label_small<T, 128, 64>);
         return launch_status();
     }
-    if (a.n * p.splits > kBatch * 2) return PIN_ERR_UNSUPPORTED;   // (n of a batch, or n < kFull and few parts)
     if (p.lanes > 0) {
         if (p.lanes == 1) launch_lanes<T, 1>(a);
         else if (p.lanes == 2) launch_lanes<T, 2>(a);
@@ -1354,13 +1358,14 @@ int forward_rows(const Call& a, const Plan& p) {
     return launch_status();
 }
 
-// Rows in batches: a launch has fewer than 2^32 threads.
+// Rows in batches; the batches of split rows take turns in the workspace, which the stream's order allows.
 template <class T>
 int run_forward(const Call& a) {
     const Plan p = plan_rows(a.n, a.classes, T::N, a.k);
-    for (int64_t row = 0; row < a.n; row += kBatch) {
+    const int64_t batch = batch_of(p);
+    for (int64_t row = 0; row < a.n; row += batch) {
         Call b = a;
-        b.n = a.n - row < kBatch ? a.n - row : kBatch;
+        b.n = a.n - row < batch ? a.n - row : batch;
         b.logits = (const typename T::type*)a.logits + row * a.row_stride;
         b.labels += row;
         b.out.log_prob += row;
@@ -1437,7 +1442,8 @@ int64_t pin_label_logprob_workspace_bytes(int64_t n, int64_t classes, int32_t dt
         return PIN_ERR_ARG;
     if (n == 0 || classes <= kSmall) return 0;
     const Plan p = plan_rows(n, classes, dtype == PIN_TYPE_F32 ? F32::N : F16::N, top_k);
-    return p.lanes > 0 || p.nch > 0 || p.alone > 0 ? 0 : n * p.splits * (16 + (top_k > 0 ? 256 : 0));
+    const int64_t rows = n < batch_of(p) ? n : batch_of(p);
+    return p.lanes > 0 || p.nch > 0 || p.alone > 0 ? 0 : rows * p.splits * (16 + (top_k > 0 ? 256 : 0));
 }
 
 int pin_label_logprob(const void* logits, int32_t dtype, int64_t n, int64_t classes, int64_t row_stride,

@@ -187,3 +187,15 @@ def test_versions_of_what_is_written():
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.backward()
     assert touched([]) == 0 and touched([p, 3]) == -1 and touched((p,)) == -1
+
+
+def test_workspace_of_many_split_rows():
+    """Rows that are split come in batches of fewer than 2^24 parts, which share one workspace."""
+    ws = _lib.load().pin_label_logprob_workspace_bytes
+    for kind, size, c in [(0, 4, 524280), (2, 2, 524280), (2, 2, 300001), (0, 4, 140001)]:
+        one = ws(1 << 12, c, kind, 4) // (1 << 12)
+        assert one > 0 and one % 272 == 0 and ws(1 << 12, c, kind, 0) * 17 == one << 12
+        parts = one // 272
+        assert 1 < parts <= 64
+        for n in ((1 << 24) // parts, (1 << 24) // parts + 1, 1 << 40):
+            assert ws(n, c, kind, 4) == ((1 << 24) - 1) // parts * one

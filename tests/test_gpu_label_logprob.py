@@ -347,6 +347,20 @@ def test_more_rows_than_one_launch_takes(dev):
     assert torch.equal(dz[-5:], dz[:1].expand(5, 5)) and bool(dz.any())
 
 
+@pytest.mark.parametrize("n,k", [(1 << 18, 0), ((1 << 18) + 5, 0), ((1 << 18) + 5, 3)])
+def test_more_split_rows_than_one_launch_takes(dev, n, k):
+    """Rows of 64 parts each (one row's memory), 2^24 parts and more: every row as the first, and as alone."""
+    c = 524280
+    row, y = make(1, c, torch.bfloat16, dev, ignore_some=False)
+    got = P.label_log_probs(row.expand(n, c), y.expand(n), top_k=k)
+    for t in got:
+        assert torch.equal(t, t[:1].expand(n, *t.shape[1:]))
+    want, tol = reference(row.cpu(), y.cpu().numpy(), k)
+    near(got.log_prob[:1], want["lp"], tol["lp"], "log_prob")
+    near(got.entropy[-1:], want["ent"], tol["ent"], "entropy")
+    np.testing.assert_array_equal(got.top_index[-1:].cpu().numpy(), want["idx"])
+
+
 def test_gradient_through_other_layouts(dev):
     """Logits that are a transposed, sliced or expanded leaf: the gradient comes back in the leaf's layout."""
     logits, y = make(6, 40, torch.float32, dev, ignore_some=False)
