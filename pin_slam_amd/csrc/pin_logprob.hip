@@ -872,6 +872,7 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
         }
 #pragma unroll
         for (int c = 0; c < NCH; ++c) forget(q[c]);
+        float ps = 0.f, pt = 0.f;   // a part's sums by themselves: the chains of a row's stay below a hundred terms
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             if (c > 0 && u0 + c * 256 >= u1) break;
@@ -881,10 +882,12 @@ k_label_row(const typename T::type* __restrict__ logits, int classes, int64_t ro
             for (int i = 0; i < T::N; ++i) {
                 const float x = fmaxf(fmaf(v[i], kL, -ml), kFloor);
                 const float e = __builtin_amdgcn_exp2f(x);
-                s += e;
-                t = fmaf(e, x, t);
+                ps += e;
+                pt = fmaf(e, x, pt);
             }
         }
+        s += ps;
+        t += pt;
     }
     put_fours(m, s_m.sup);
     const float wm = wave_max(m);

@@ -321,6 +321,29 @@ def test_an_ignored_row_masked_by_a_finite_value_passes_no_gradient(dev):
             assert not bool(dz[1].any()) and bool(torch.isfinite(dz).all())
 
 
+@pytest.mark.parametrize("kind,c", [("f32", 131000), ("f16", 131072), ("bf16", 131072), ("bf16", 262000)])
+def test_longest_rows_of_one_workgroup(dev, c, kind):
+    """A workgroup's longest rows, many of them: nearly flat ones, whose sums take the most
+    terms of one size, at several heights (the f32 values of the terms go by it: at 1360, 2736 and 3408 they are 1 and
+    nearly 2^-15 more or less, which a chain of a thousand terms rounds off or up each time, 254 u in all), a range held
+    by a finite mask."""
+    g = torch.Generator().manual_seed(c)
+    base = torch.randn((c,), generator=g)
+    rows = [base * 0.0, base * 0.0 + 1360.0, base * 0.0 + 2736.0, base * 0.0 + 3408.0, base * 1e-3, 0.1 + base * 0.05, 37.7 + torch.linspace(0.0, 0.4, c), -911.3 - torch.linspace(0.0, 0.3, c),
+            base, 3 * base, torch.where(torch.arange(c) < c // 2, -1e10, base), -3e7 + 0.3 * base, 5e6 + torch.linspace(0.0, 2.0, c)]
+    z = torch.stack(rows).to(TYPES[kind]) if kind != "f16" else torch.stack(rows[:10]).to(TYPES[kind])
+    n = z.shape[0]
+    y = torch.randint(0, c, (n,), generator=g)
+    for k in (0, 3):
+        want, tol = reference(z, y.numpy(), k)
+        got = P.label_log_probs(z.to(dev)[:, None].expand(n, 300, c), y.to(dev)[:, None].expand(n, 300), top_k=k)
+        assert all(torch.equal(t, t[:, :1].expand(t.shape)) for t in got)
+        near(got.log_prob[:, 0], want["lp"], tol["lp"], "log_prob")
+        near(got.entropy[:, 0], want["ent"], tol["ent"], "entropy")
+        np.testing.assert_array_equal(got.top_index[:, 0].cpu().numpy(), want["idx"])
+        near(got.top_log_prob[:, 0], want["top"], tol["top"], "top_log_prob")
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("times", [1, 33])
 def test_large_values_in_one_place(dev, kind, times):
