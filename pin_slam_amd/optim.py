@@ -18,6 +18,7 @@ import torch
 from . import _lib
 
 _SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
+_INF = float("inf")
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
 
 
@@ -48,6 +49,7 @@ class _Arena:
         self.v = torch.zeros((total,), dtype=kind, device=dev)
         self.exps = torch.zeros((total // _lib.ADAMW_BLOCK, 2), dtype=torch.int16, device=dev) if bits == 8 else None
         self.master = torch.zeros((total,), dtype=torch.float32, device=dev) if _has_master(group) else None
+        self.master_weights = group["master_weights"]
         self.held = None
         self.index = dev.index
         self.c_sizes, self.c_offsets = array("q", self.sizes), array("q", self.offsets)
@@ -127,24 +129,24 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: a tensor lr must be one float32 on the parameters' device, with capturable=True")
 
     @staticmethod
-    def _check_rates(group):
-        lr, (b1, b2) = group["lr"], group["betas"]
-        if not 0.0 <= lr < float("inf"):
+    def _check_rates(group, lr):
+        b1, b2 = group["betas"]
+        if (0.0 <= lr < _INF and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and 0.0 <= group["eps"] < _INF
+                and 0.0 <= group["weight_decay"] < _INF and group["state_bits"] in _STATE_KEYS):
+            return
+        if not 0.0 <= lr < _INF:
             raise ValueError(f"AdamW: lr must be >= 0 (got {lr})")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW: betas must be in [0, 1) (got {group['betas']})")
-        if not 0.0 <= group["eps"] < float("inf") or not 0.0 <= group["weight_decay"] < float("inf"):
-            raise ValueError(f"AdamW: eps and weight_decay must be >= 0 (got {group['eps']}, {group['weight_decay']})")
         if group["state_bits"] not in _STATE_KEYS:
             raise ValueError(f"AdamW: state_bits must be 32 or 8 (got {group['state_bits']})")
+        raise ValueError(f"AdamW: eps and weight_decay must be >= 0 (got {group['eps']}, {group['weight_decay']})")
 
     def _check_group(self, group):
         params = group["params"]
         if isinstance(group["lr"], torch.Tensor):
             self._check_lr(group["lr"], params[0].device)
-            self._check_rates({**group, "lr": 0.0})
-        else:
-            self._check_rates(group)
+        self._check_rates(group, 0.0 if isinstance(group["lr"], torch.Tensor) else group["lr"])
         spans = []
         for p in params:
             if p.dtype not in _lib.TYPES:
@@ -219,16 +221,26 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []
-        for gi, group in enumerate(self.param_groups):   # everything is checked before anything is stepped
-            if not group["params"] or not (self.capturable or any(p.grad is not None for p in group["params"])):
+        # everything is checked before anything is stepped, and the groups before any state is made
+        groups, work = [], []
+        for gi, group in enumerate(self.param_groups):
+            params = group["params"]
+            if not params or not (self.capturable or params[0].grad is not None or any(p.grad is not None for p in params)):
                 continue
-            _lib.require_device(group["params"][0])
+            _lib.require_device(params[0])
             if not self.capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: capturing a step needs capturable=True (the step count is on the host)")
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor):
+                self._check_lr(lr, params[0].device)
+                lr = 0.0
+            self._check_rates(group, lr)
+            arena = self._arenas.get(gi)
+            if arena is not None and (arena.bits != group["state_bits"] or arena.master_weights != group["master_weights"]):
+                raise RuntimeError("AdamW: state_bits or master_weights changed after a group's first step")
+            groups.append((gi, group))
+        for gi, group in groups:
             arena = self._arena(gi)
-            if isinstance(group["lr"], torch.Tensor):
-                self._check_lr(group["lr"], arena.device)
             work.append((gi, group, arena, self._gather(arena, group)))
         for gi, group, arena, todo in work:
             with _lib.on_device(arena.device):
@@ -319,7 +331,7 @@ class AdamW(torch.optim.Optimizer):
             for key in ("state_bits", "master_weights"):
                 if mine[key] != saved[key]:
                     raise ValueError(f"AdamW: the saved state has {key} {saved[key]}, this optimiser {mine[key]}")
-            self._check_rates({**saved, "lr": float(saved["lr"])})
+            self._check_rates(saved, float(saved["lr"]))
         plan = []
         k = 0
         for gi, group in enumerate(self.param_groups):

@@ -767,6 +767,36 @@ def test_queries_between_replays(dev):
         assert all(torch.equal(a, b) for a, b in zip(after, fresh))
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+def test_rates_changed_later_are_checked_before_any_group_steps(dev, capturable):
+    """A group that is refused leaves the others as they were, and the next good step goes on from there."""
+    def build():
+        a, b = tensors([500, 20], torch.bfloat16, dev), tensors([300], torch.float32, dev, 1)
+        for ps in (a, b):
+            set_grads(ps, 3)
+        return a + b, P.AdamW([dict(params=a, master_weights=True), dict(params=b, state_bits=8)], capturable=capturable,
+                              **HYPER)
+
+    (params, opt), (others, ref) = build(), build()
+    opt.step()
+    ref.step()
+    for key, bad in (("lr", -1.0), ("lr", math.nan), ("betas", (0.9, 1.0)), ("betas", (-0.1, 0.9)), ("eps", -1e-3),
+                     ("weight_decay", math.inf), ("state_bits", 16), ("state_bits", 32), ("master_weights", True)):
+        group = opt.param_groups[1]
+        kept, group[key] = group[key], bad
+        versions = [p._version for p in params]
+        with pytest.raises((ValueError, RuntimeError)):
+            opt.step()
+        group[key] = kept
+        assert [p._version for p in params] == versions
+        assert all(torch.equal(p, q) for p, q in zip(params, others))
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [1, 1, 1]
+    opt.step()
+    ref.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, others))
+    assert all(torch.equal(x, y) for gi in (0, 1) for x, y in zip(opt.moments(gi), ref.moments(gi)))
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
