@@ -310,20 +310,24 @@ class AdamW(torch.optim.Optimizer):
         return self._arena(group).master
 
     def state_dict(self):
-        saved = super().state_dict()
-        k, steps = 0, {}
-        for gi, group in enumerate(self.param_groups):
-            arena = self._arenas.get(gi)
-            for i in range(len(group["params"])):
-                if arena is not None:
-                    steps[k] = arena.steps[i] if arena.step_dev is None else int(arena.step_dev)
-                k += 1
-        saved["state"] = {k: {"step": steps[k], **one} for k, one in saved["state"].items()}
-        return saved
+        kept = dict(self.state)
+        for gi, arena in self._arenas.items():
+            step = None if arena.step_dev is None else int(arena.step_dev)
+            for p, n in zip(self.param_groups[gi]["params"], arena.steps):   # the counts as torch's hooks expect them
+                self.state[p] = {"step": n if step is None else step, **kept[p]}
+        try:
+            return super().state_dict()
+        finally:
+            self.state.update(kept)
 
     def load_state_dict(self, state_dict):
         """Takes a state_dict of an AdamW with the same groups (its state_bits and master_weights too).  State that is
-        there already is written where it lies, so a graph that holds a step goes on from what was loaded."""
+        there already is written where it lies, so a graph that holds a step goes on from what was loaded.  torch's
+        hooks of loading and saving run as they do around its own optimisers."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the saved state has other parameter groups")
@@ -387,3 +391,5 @@ class AdamW(torch.optim.Optimizer):
             arena.together = len(set(arena.steps)) == 1
         for gi, step in by.items():
             self._arenas[gi].step_dev.fill_(step)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)

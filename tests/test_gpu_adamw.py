@@ -410,6 +410,46 @@ def test_load_refuses_what_does_not_fit(dev):
         P.AdamW(tensors([300], torch.float32, dev), state_bits=8).load_state_dict(bad)
 
 
+def test_hooks_of_saving_and_loading(dev):
+    """torch's hooks see what they see of its own optimisers: the whole saved state, the state to load before it is taken
+    (and may put another in its place), the optimiser after."""
+    def build():
+        p = tensors([300, 20], torch.float32, dev)
+        return p, P.AdamW(p, state_bits=8, **HYPER)
+
+    a, opt = build()
+    set_grads(a, 1)
+    opt.step()
+    seen = []
+    opt.register_state_dict_pre_hook(lambda o: seen.append(("save", o)))
+
+    def after(o, saved):
+        seen.append(("saved", [s["step"] for s in saved["state"].values()]))
+        return {**saved, "extra": 7}
+
+    opt.register_state_dict_post_hook(after)
+    saved = opt.state_dict()
+    assert seen == [("save", opt), ("saved", [1, 1])] and saved["extra"] == 7
+    assert all("step" not in opt.state[p] for p in a)
+    b, other = build()
+    calls = []
+
+    def before(o, d):
+        calls.append(o)
+        assert d is not saved and d["extra"] == 7
+        groups = [{**g, "lr": 0.5} for g in d["param_groups"]]
+        return {**d, "param_groups": groups}
+
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(lambda o: calls.append(o.param_groups[0]["lr"]))
+    other.load_state_dict(saved)
+    assert calls == [other, 0.5] and saved["param_groups"][0]["lr"] == HYPER["lr"]
+    assert all(torch.equal(x, y) for x, y in zip(opt.moments(), other.moments()))
+    copied = copy.deepcopy(other)
+    copied.load_state_dict(copied.state_dict())   # (a copy has no hooks)
+    assert len(calls) == 2
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_and_replayed(dev, bits):
     """A captured step counts on: replays with new gradients and a new lr equal eager steps of another optimiser."""
