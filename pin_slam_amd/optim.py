@@ -19,6 +19,7 @@ from . import _lib
 
 _SALT_SEED, _SALT_GROUP = 0x9E3779B1, 0xBB67AE85
 _INF = float("inf")
+_RATES = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights")
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exponents")}
 
 
@@ -328,10 +329,15 @@ class AdamW(torch.optim.Optimizer):
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
             state_dict = state_dict if changed is None else changed
+        if "state" not in state_dict or "param_groups" not in state_dict:
+            raise ValueError("AdamW: the saved state has no state or no param_groups: not an optimiser's")
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the saved state has other parameter groups")
         for mine, saved in zip(self.param_groups, groups):
+            for key in _RATES:
+                if key not in saved:
+                    raise ValueError(f"AdamW: the saved state's groups have no {key} (another optimiser's?)")
             for key in ("state_bits", "master_weights"):
                 if mine[key] != saved[key]:
                     raise ValueError(f"AdamW: the saved state has {key} {saved[key]}, this optimiser {mine[key]}")
@@ -351,8 +357,8 @@ class AdamW(torch.optim.Optimizer):
                     dtype = {"exponents": torch.int16, "master": torch.float32}.get(key, kind)
                     if key not in one or tuple(one[key].shape) != shape or one[key].dtype != dtype:
                         raise ValueError(f"AdamW: the saved {key} of parameter {k - 1} is not a {dtype} of {shape}")
-                if int(one["step"]) < 0:
-                    raise ValueError(f"AdamW: the saved step of parameter {k - 1} is {one['step']}")
+                if int(one.get("step", -1)) < 0:
+                    raise ValueError(f"AdamW: the saved step of parameter {k - 1} is {one.get('step')}")
                 plan.append((gi, i, p, want, one))
             if self.capturable and len({int(o["step"]) for g, _, _, _, o in plan if g == gi}) > 1:
                 raise ValueError("AdamW: with capturable=True the parameters of a group share one step")

@@ -450,6 +450,27 @@ def test_hooks_of_saving_and_loading(dev):
     assert len(calls) == 2
 
 
+def test_load_names_what_another_optimisers_state_lacks(dev):
+    p = tensors([300], torch.float32, dev)
+    set_grads(p, 1)
+    opt = P.AdamW(p, **HYPER)
+    theirs = torch.optim.AdamW(tensors([300], torch.float32, dev), foreach=False)
+    theirs.param_groups[0]["params"][0].grad = torch.ones(300, device=dev)
+    theirs.step()
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.load_state_dict(theirs.state_dict())
+    opt.step()
+    saved = opt.state_dict()
+    for bad in ({}, {"state": {}}, {"param_groups": saved["param_groups"]}):
+        with pytest.raises(ValueError, match="param_groups"):
+            opt.load_state_dict(bad)
+    with pytest.raises(ValueError, match="betas"):
+        opt.load_state_dict({**saved, "param_groups": [{k: v for k, v in saved["param_groups"][0].items() if k != "betas"}]})
+    with pytest.raises(ValueError, match="step"):
+        opt.load_state_dict({**saved, "state": {0: {k: v for k, v in saved["state"][0].items() if k != "step"}}})
+    assert opt.state_dict()["state"][0]["step"] == 1
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_and_replayed(dev, bits):
     """A captured step counts on: replays with new gradients and a new lr equal eager steps of another optimiser."""
