@@ -48,8 +48,8 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
         z = z.contiguous()
     if z.is_neg():
         z = z.resolve_neg()
-    if y.dtype != torch.int64 or not y.is_contiguous():
-        y = y.to(torch.int64).contiguous()
+    if y.dtype != torch.int64 or not y.is_contiguous() or y.is_neg():
+        y = y.to(torch.int64).contiguous().resolve_neg()
     lp, ent, tlp, tidx = _lib.torch_fn("pin_torch_label")(
         _lib.address("pin_label_logprob_workspace_bytes"), _lib.address("pin_label_logprob"),
         _lib.address("pin_label_logprob_bwd"), z, y, k, int(ignore_index),

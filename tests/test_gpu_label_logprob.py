@@ -634,6 +634,18 @@ def test_views_that_negate_and_forward_mode(dev):
         P.label_log_probs(fwd.make_dual(logits, torch.ones_like(logits)), y)
 
 
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.int16, torch.int8])
+def test_labels_that_are_a_negating_view(dev, kind):
+    logits, y = make(9, 100, torch.float32, dev)
+    n = torch._neg_view((-y).to(kind))
+    x = logits.detach().clone().requires_grad_(True)
+    want, got = P.label_log_probs(x, y, top_k=2), P.label_log_probs(x, n, top_k=2)
+    assert n.is_neg() and all(torch.equal(a, b) for a, b in zip(got, want))
+    a, = torch.autograd.grad(want.log_prob.sum(), x)
+    b, = torch.autograd.grad(got.log_prob.sum(), x)
+    assert torch.equal(a, b)
+
+
 def test_the_node_in_torchs_graph(dev):
     """What torch does with any operator's results: kept graphs, results changed in place, hooks, checkpoints, anomaly
     checks, results and graphs that go without a backward pass."""
