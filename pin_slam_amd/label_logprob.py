@@ -12,6 +12,7 @@ import torch
 
 from . import _lib
 
+_NO_CLASS = (1 << 63) - 1
 LabelLogProbs = namedtuple("LabelLogProbs", ["log_prob", "entropy", "top_log_prob", "top_index"])
 
 
@@ -41,6 +42,9 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
     k = int(top_k)
     if not 0 <= k <= min(c, _lib.LABEL_TOP_MAX):
         raise ValueError(f"label_log_probs: top_k must be 0 to min(classes, {_lib.LABEL_TOP_MAX}) (got {top_k})")
+    ignore = int(ignore_index)
+    if not -(1 << 63) <= ignore < 1 << 63:
+        raise ValueError(f"label_log_probs: ignore_index must fit in 64 bits with a sign (got {ignore_index})")
     z, y = logits, labels
     if logits.dim() != 2:
         z, y = logits.reshape(labels.numel(), c), labels.reshape(-1)
@@ -48,11 +52,14 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
         z = z.contiguous()
     if z.is_neg():
         z = z.resolve_neg()
+    if y.dtype == torch.uint64:   # beyond int64: no class, and not what ignore_index would be there
+        y = y.to(torch.int64)
+        y = torch.where(y < 0, _NO_CLASS - (ignore == _NO_CLASS), y)
     if y.dtype != torch.int64 or not y.is_contiguous() or y.is_neg():
         y = y.to(torch.int64).contiguous().resolve_neg()
     lp, ent, tlp, tidx = _lib.torch_fn("pin_torch_label")(
         _lib.address("pin_label_logprob_workspace_bytes"), _lib.address("pin_label_logprob"),
-        _lib.address("pin_label_logprob_bwd"), z, y, k, int(ignore_index),
+        _lib.address("pin_label_logprob_bwd"), z, y, k, ignore,
         1 if logits.requires_grad and torch.is_grad_enabled() else 0)
     if logits.dim() != 2:
         lead = labels.shape

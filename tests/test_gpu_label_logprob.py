@@ -634,6 +634,25 @@ def test_views_that_negate_and_forward_mode(dev):
         P.label_log_probs(fwd.make_dual(logits, torch.ones_like(logits)), y)
 
 
+def test_unsigned_labels(dev):
+    """Labels of 64 bits without a sign: those beyond int64 are no class, whatever ignore_index is."""
+    logits, _ = make(6, 40, torch.float32, dev)
+    y = torch.tensor([3, 39, 40, 0, 5, 7], device=dev)
+    want = P.label_log_probs(logits, y, ignore_index=5)
+    for kind in (torch.uint8, torch.uint16, torch.uint32, torch.uint64):
+        got = P.label_log_probs(logits, y.to(kind), ignore_index=5)
+        assert torch.equal(torch.nan_to_num(got.log_prob, nan=7.0), torch.nan_to_num(want.log_prob, nan=7.0))
+    far = torch.from_numpy(np.array([2 ** 64 - 100, 2 ** 64 - 1, 2 ** 63, 2 ** 63 - 1, 2, 39], dtype=np.uint64)).to(dev)
+    for ignore in (IGNORE, -1, -2 ** 63):
+        got = P.label_log_probs(logits, far, ignore_index=ignore).log_prob
+        assert torch.isnan(got).tolist() == [True] * 4 + [False] * 2
+    got = P.label_log_probs(logits, far, ignore_index=2 ** 63 - 1).log_prob
+    assert torch.isnan(got).tolist() == [True] * 3 + [False] * 3 and float(got[3]) == 0.0
+    for ignore in (2 ** 63, 2 ** 64 - 100, -2 ** 63 - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            P.label_log_probs(logits, far, ignore_index=ignore)
+
+
 @pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.int16, torch.int8])
 def test_labels_that_are_a_negating_view(dev, kind):
     logits, y = make(9, 100, torch.float32, dev)
