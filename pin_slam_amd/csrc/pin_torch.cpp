@@ -8,6 +8,7 @@
 // pin_torch_label: label_log_probs' outputs, launch and node in torch's graph, in one call.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -26,6 +27,14 @@ bool as_taken(const at::Tensor& t, c10::ScalarType type, int64_t device, int64_t
            !t.is_neg() && t.scalar_type() == type && (device < 0 ? t.is_cpu() : t.is_cuda() && t.get_device() == device) &&
            t.numel() == size && t.is_contiguous();
 }
+
+// A tensor with memory of its own that the kernels may read: no wrapper of a transform, a trace or another program's class.
+bool has_memory(const at::Tensor& t) {
+    const c10::DispatchKeySet keys = t.key_set();
+    return t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() && !keys.has(c10::DispatchKey::Functionalize) &&
+           !keys.has(c10::DispatchKey::FuncTorchBatched) && !keys.has(c10::DispatchKey::FuncTorchGradWrapper);
+}
+bool transformed() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode); }
 
 // The gradient of label_log_probs as a node of torch's graph: the engine runs it on a thread of its own, where
 // the same in Python takes longer (forward and gradient of 16384 x 1003 f16 105 us, with this node 73).
@@ -56,6 +65,9 @@ struct LabelNode : torch::autograd::Node {
 
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
+        bool plain = !transformed();
+        for (const at::Tensor& g : grads) plain = plain && (!g.defined() || has_memory(g));
+        TORCH_CHECK_NOT_IMPLEMENTED(plain, "label_log_probs: batched gradients and torch.func's transforms are not implemented");
         at::Tensor z = logits.unpack(), y = labels.unpack(), idx = k > 0 ? top.unpack() : at::Tensor();
         at::Tensor dz;
         {
@@ -93,6 +105,8 @@ struct NoInterpreter {
 void label_forward(LabelWorkspace workspace, LabelFwd forward, LabelBwd backward, const at::Tensor& z, const at::Tensor& y,
                    int64_t k, int64_t ignore, bool grad, at::Tensor& lp, at::Tensor& ent, at::Tensor& top_lp,
                    at::Tensor& top_idx) {
+    TORCH_CHECK_NOT_IMPLEMENTED(has_memory(z) && has_memory(y) && !transformed(),
+                                "label_log_probs: torch.func's transforms and tensors without memory are not implemented");
     TORCH_CHECK_NOT_IMPLEMENTED(!z._fw_grad(0).defined(), "label_log_probs: forward-mode differentiation is not implemented");
     const int64_t n = z.size(0), c = z.size(1);
     const c10::DeviceGuard device(z.device());

@@ -25,7 +25,9 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
     is ignore_index have log_prob 0 and pass no gradient through it.  Classes at -inf have
     probability 0; a row with nothing else has log_prob -inf, entropy 0 and gradient 0, a row with
     a NaN or +inf has NaN and top_index -1, a label outside [0, C) has log_prob NaN.  Rows may be
-    strided (a slice of padded logits is read where it lies)."""
+    strided (a slice of padded logits is read where it lies).  torch.func's transforms (vmap, grad,
+    jvp, functionalize), forward-mode differentiation and fake tensors are refused; torch.compile
+    breaks its graph here and calls this eagerly."""
     _lib.require_device(logits)
     if logits.dtype not in _lib.TYPES:
         raise ValueError(f"label_log_probs: logits must be float32, float16 or bfloat16 (got {logits.dtype})")

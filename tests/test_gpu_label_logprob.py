@@ -665,6 +665,57 @@ def test_labels_that_are_a_negating_view(dev, kind):
     assert torch.equal(a, b)
 
 
+def test_transforms_are_refused(dev):
+    """torch.func's transforms and tensors without memory: an error before any launch, and nothing is left behind."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    logits, y = make(6, 70, torch.float32, dev, ignore_some=False)
+    many, ys = logits.view(2, 3, 70), y.view(2, 3)
+    loss = lambda z: P.label_log_probs(z, y).log_prob.sum()   # noqa: E731
+    whole = lambda _: loss(logits)   # noqa: E731  (what it reads is no argument of the transform)
+    calls = [lambda: torch.func.grad(loss)(logits), lambda: torch.func.vjp(loss, logits), lambda: torch.func.grad(lambda z: loss(logits) + z.sum())(logits),
+             lambda: torch.func.vmap(lambda z, t: P.label_log_probs(z, t).log_prob)(many, ys),
+             lambda: torch.func.vmap(lambda t: P.label_log_probs(logits[:3], t).log_prob)(ys),
+             lambda: torch.func.vmap(lambda z: P.label_log_probs(z, ys[0], top_k=2).top_log_prob)(many),
+             lambda: torch.func.vmap(whole)(many), lambda: torch.func.jvp(loss, (logits,), (torch.ones_like(logits),)),
+             lambda: torch.func.functionalize(loss)(logits), lambda: torch.func.hessian(loss)(logits)]
+    for call in calls:
+        with pytest.raises(NotImplementedError, match="torch.func|forward-mode"):
+            call()
+    x = logits.detach().clone().requires_grad_(True)
+    r = P.label_log_probs(x, y, top_k=2)
+    for out, up in ((r.log_prob, torch.ones((3, 6), device=dev)), (r.top_log_prob, torch.ones((3, 6, 2), device=dev))):
+        with pytest.raises(NotImplementedError, match="batched gradients"):
+            torch.autograd.grad(out, x, up, is_grads_batched=True, retain_graph=True)
+    dz, = torch.autograd.grad(r.log_prob.sum(), x)   # the graph is as it was
+    assert bool(dz.any())
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = mode.from_tensor(logits)
+        with pytest.raises(NotImplementedError, match="without memory"):
+            P.label_log_probs(fake, mode.from_tensor(y))
+    want, tol = reference(logits.cpu(), y.cpu().numpy(), 2)
+    near(P.label_log_probs(logits, y, top_k=2).log_prob, want["lp"], tol["lp"], "log_prob")
+
+
+def test_under_torch_compile(dev):
+    """The graph breaks there: values and gradients are the eager call's."""
+    logits, y = make(30, 70, torch.float32, dev)
+
+    def loss(z, t):
+        r = P.label_log_probs(z * 2.0, t, top_k=2)
+        return -r.log_prob.sum() + 0.1 * r.entropy.sum() + r.top_log_prob[:, 1].sum()
+
+    for backend in ("eager", "aot_eager"):
+        torch._dynamo.reset()
+        fast = torch.compile(loss, backend=backend)
+        for turn in range(3):
+            x, q = (logits.detach().clone().add_(turn).requires_grad_(True) for _ in range(2))
+            a, b = loss(x, y), fast(q, y)
+            a.backward()
+            b.backward()
+            assert torch.equal(a, b) and torch.equal(x.grad, q.grad)
+    torch._dynamo.reset()
+
+
 def test_the_node_in_torchs_graph(dev):
     """What torch does with any operator's results: kept graphs, results changed in place, hooks, checkpoints, anomaly
     checks, results and graphs that go without a backward pass."""
