@@ -705,6 +705,40 @@ def test_a_training_step_of_the_class_head(dev):
         assert float((x - y).abs().max()) <= 0.1 * 5 * 0.01
 
 
+def test_each_step_of_the_class_heads_training(dev):
+    """Loss, gradient and step of the two operators: torch's AdamW, fed the gradients that this run's loss gave, goes the
+    same way parameter by parameter.  A step is off by 14 u of its update (at most lr) and 3 u of the parameter on either
+    side, and five of them add up: 30 u |p| + 140 u lr, 1.8e-6 |p| + 8.4e-8.  (A bias correction or decay that is wrong
+    by a thousandth moves a parameter by 1e-5.)"""
+    cfg = P.Config(device=dev)
+    torch.manual_seed(12)
+    dec = P.Decoder(cfg, cfg.geo_mlp_hidden_dim, cfg.geo_mlp_level, 20)
+    feats = torch.nn.Parameter(torch.randn((4000, 11), device=dev))
+    y = torch.randint(0, 20, (4000,), device=dev)
+    y[::7] = -100
+    mine = [feats, *dec.parameters()]
+    theirs = [torch.nn.Parameter(p.detach().clone()) for p in mine]
+    hyper = dict(lr=0.01, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    opt, ref = P.AdamW(mine, **hyper), torch.optim.AdamW(theirs, foreach=False, **hyper)
+    kept = (y != -100).sum()
+    losses = []
+    for _ in range(5):
+        opt.zero_grad()
+        r = dec.sem_label_log_prob(feats, y, top_k=3)
+        loss = -r.log_prob.sum() / kept + 0.1 * r.entropy.mean()
+        loss.backward()
+        before = [p.detach().clone() for p in mine]
+        for p, q in zip(mine, theirs):
+            q.grad = p.grad.clone()
+        opt.step()
+        ref.step()
+        losses.append(float(loss))
+        for p, q, b in zip(mine, theirs, before):
+            torch.testing.assert_close(p.detach(), q.detach(), rtol=1.8e-6, atol=8.4e-8)
+            assert float((p.detach() - b).abs().max()) > 1e-3   # it moved
+    assert all(math.isfinite(x) for x in losses)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_captured_training_step(dev, bits):
     """Loss, gradient into the leaf's own .grad and step in one graph, replayed between eager work, against the same calls

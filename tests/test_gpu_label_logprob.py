@@ -309,6 +309,19 @@ def test_large_finite_masks_of_many_rows(dev, c, times, kind):
         check(z.repeat(times, 1).to(dev), y.repeat(times).to(dev), k)
 
 
+@pytest.mark.parametrize("c,times", [(20, 1), (100, 1), (700, 1), (700, 700), (9001, 1), (20003, 43), (131073, 1)])
+def test_maxima_about_the_size_beyond_which_they_are_subtracted_first(dev, c, times):
+    """Rows whose classes, threads and parts lie on both sides of 2^20, in either sign."""
+    g = torch.Generator().manual_seed(c)
+    base = torch.randn((c,), generator=g)
+    at, half = float(1 << 20), torch.arange(c) < c // 2
+    rows = [s * at + d + w * base for s in (-1, 1) for d in (-3.0, 0.0, 3.0) for w in (0.0, 1.0)]
+    rows += [torch.where(half, s * at - 2.0 + 0.5 * base, s * at + 2.0 + 0.5 * base) for s in (-1, 1)]
+    z, y = torch.stack(rows), torch.randint(0, c, (len(rows),), generator=g)
+    for k in (0, 2):
+        check(z.repeat(times, 1).to(dev), y.repeat(times).to(dev), k)
+
+
 def test_an_ignored_row_masked_by_a_finite_value_passes_no_gradient(dev):
     """What a padded row leaves in the gradient of the layer before it: nothing."""
     for c in (20, 700, 9001, 131073):
