@@ -166,6 +166,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _arena(self, gi):
         group = self.param_groups[gi]
+        gi %= len(self.param_groups)   # (the last group is also number -1)
         arena = self._arenas.get(gi)
         if arena is None:
             for p in group["params"]:

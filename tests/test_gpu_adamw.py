@@ -892,6 +892,28 @@ def test_rates_changed_later_are_checked_before_any_group_steps(dev, capturable)
     assert all(torch.equal(x, y) for gi in (0, 1) for x, y in zip(opt.moments(gi), ref.moments(gi)))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_counted_from_the_end(dev, bits):
+    """moments(-1) is the last group's, and asking changes nothing."""
+    a, b = tensors([500], torch.float32, dev), tensors([300, 20], torch.bfloat16, dev, 1)
+    opt = P.AdamW([dict(params=a), dict(params=b, master_weights=True)], state_bits=bits, **HYPER)
+    for t in (1, 2):
+        set_grads(a + b, t)
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    for gi in (1, 0):
+        assert all(torch.equal(x, y) and bool(x.any()) for x, y in zip(opt.moments(gi), opt.moments(gi - 2)))
+        assert opt.offsets(gi) == opt.offsets(gi - 2)
+    assert torch.equal(opt.master(1), opt.master(-1)) and opt.master(0) is None and opt.master(-2) is None
+    again = opt.state_dict()
+    for k, one in saved["state"].items():
+        assert one["step"] == again["state"][k]["step"] == 2
+        assert all(torch.equal(one[key], again["state"][k][key]) for key in one if key != "step")
+    for bad in (2, -3):
+        with pytest.raises(IndexError):
+            opt.moments(bad)
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
