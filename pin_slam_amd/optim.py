@@ -164,6 +164,10 @@ class AdamW(torch.optim.Optimizer):
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: two parameters share memory")
 
+    def _show(self, arena, group):
+        for i, p in enumerate(group["params"]):
+            self.state[p] = arena.views(i, p.shape)
+
     def _arena(self, gi):
         group = self.param_groups[gi]
         gi %= len(self.param_groups)   # (the last group is also number -1)
@@ -174,8 +178,14 @@ class AdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: run one step before capturing one (it makes the state)")
             arena = self._arenas[gi] = _Arena(group, self.capturable)
-            for i, p in enumerate(group["params"]):
-                self.state[p] = arena.views(i, p.shape)
+            self._show(arena, group)
+        elif group["params"] and group["params"][0] not in self.state:   # state was emptied: torch's optimisers begin anew
+            if not arena.fits(group) or any(p in self.state for p in group["params"]):
+                raise RuntimeError("AdamW: parameters were added to or taken from a group after its first step")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: run one step before capturing one (it makes the state)")
+            arena.start(group["params"])
+            self._show(arena, group)
         if len(arena.sizes) != len(group["params"]):
             raise RuntimeError("AdamW: parameters were added to or taken from a group after its first step")
         return arena
@@ -316,7 +326,8 @@ class AdamW(torch.optim.Optimizer):
         for gi, arena in self._arenas.items():
             step = None if arena.step_dev is None else int(arena.step_dev)
             for p, n in zip(self.param_groups[gi]["params"], arena.steps):   # the counts as torch's hooks expect them
-                self.state[p] = {"step": n if step is None else step, **kept[p]}
+                if p in kept:
+                    self.state[p] = {"step": n if step is None else step, **kept[p]}
         try:
             return super().state_dict()
         finally:

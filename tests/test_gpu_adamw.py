@@ -914,6 +914,36 @@ def test_groups_counted_from_the_end(dev, bits):
             opt.moments(bad)
 
 
+@pytest.mark.parametrize("bits,capturable", [(32, False), (8, False), (8, True)])
+def test_emptied_state_begins_anew(dev, bits, capturable):
+    """Emptying or replacing opt.state, as programs do with torch's optimisers: the next step is a first step, and a
+    parameter that takes another's place in a group is refused."""
+    from collections import defaultdict
+    a, b = tensors([500, 20], torch.bfloat16, dev), None
+    opt = P.AdamW(a, state_bits=bits, master_weights=True, capturable=capturable, **HYPER)
+    for way in ("clear", "replace"):
+        for t in (1, 2):
+            set_grads(a, t)
+            opt.step()
+        b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+        ref = P.AdamW(b, state_bits=bits, master_weights=True, capturable=capturable, **HYPER)
+        if way == "clear":
+            opt.state.clear()
+        else:
+            opt.state = defaultdict(dict)
+        assert opt.state_dict()["state"] == {}
+        for t in (1, 2):
+            set_grads(a, 5 + t)
+            set_grads(b, 5 + t)
+            opt.step()
+            ref.step()
+            assert all(torch.equal(p, q) for p, q in zip([*a, *opt.moments(), opt.master()], [*b, *ref.moments(), ref.master()]))
+        assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2]
+    opt.param_groups[0]["params"][0] = b[0]
+    with pytest.raises(RuntimeError, match="added to or taken from"):
+        opt.step()
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
