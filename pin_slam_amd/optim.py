@@ -70,6 +70,7 @@ class _Arena:
         if self.master is not None:
             for p, a, n in zip(params, self.offsets, self.sizes):
                 self.master[a:a + n] = p.detach().reshape(-1)
+        self.wide = [p.dtype == torch.float32 for p in params]
         self.steps = [0] * len(params)
         self.together = True              # all of them are the same
 
@@ -198,6 +199,8 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: a parameter was reshaped or moved after its first step")
         if g.dtype != p.dtype or g.device != arena.device or p.dtype not in _lib.TYPES or g.numel() != arena.sizes[i]:
             raise RuntimeError(f"AdamW: a {p.dtype} parameter on {p.device} has a {g.dtype} gradient on {g.device}")
+        if arena.master_weights and (p.dtype == torch.float32) != arena.wide[i]:   # its copy is another's, or there is none
+            raise RuntimeError(f"AdamW: a parameter with a copy in 32 bits became {p.dtype} after its first step")
         if p.is_neg():
             raise RuntimeError("AdamW: a parameter is a negated view")
         return g.resolve_neg().contiguous()
@@ -210,7 +213,8 @@ class AdamW(torch.optim.Optimizer):
         if arena.together:   # the usual step: every parameter and every gradient as the kernel takes them
             ps, gs = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
             if _lib.torch_fn("pin_torch_gather")(params, n, arena.c_sizes.buffer_info()[0], arena.index, ps.buffer_info()[0],
-                                   gs.buffer_info()[0]) >= 0:
+                                   gs.buffer_info()[0]) >= 0 and not (
+                    arena.master_weights and (params[0].dtype == torch.float32) != arena.wide[0]):
                 return [(None, params[0].dtype, ps, gs)]
         grads = [p.grad for p in params]
         which = [i for i, g in enumerate(grads) if g is not None]

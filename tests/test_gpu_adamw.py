@@ -944,6 +944,49 @@ def test_emptied_state_begins_anew(dev, bits, capturable):
         opt.step()
 
 
+@pytest.mark.parametrize("first,then", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_a_parameter_that_changes_its_width_beside_its_copy_is_refused(dev, first, then):
+    """master_weights: a parameter that became 16 bits wide has no copy, or one of its first value, and one that became 32
+    bits wide would leave its copy behind; loading starts from what it is now.  Without copies the type may change."""
+    for alone in (True, False):
+        p = tensors([300] if alone else [300, 20], first, dev)
+        if not alone:
+            p[1].data = p[1].data.to(torch.float16)
+        opt = P.AdamW(p, master_weights=True, **HYPER)
+        set_grads(p, 1)
+        opt.step()
+        p[0].grad, p[0].data = None, p[0].data.to(then)
+        set_grads(p, 2)
+        before = [q.detach().clone() for q in p]
+        with pytest.raises(RuntimeError, match="copy in 32 bits became"):
+            opt.step()
+        assert all(torch.equal(x, q) for x, q in zip(before, p))
+        b = [torch.nn.Parameter(x.clone()) for x in before]
+        other = P.AdamW(b, master_weights=True, **HYPER)
+        opt.load_state_dict(other.state_dict())
+        set_grads(b, 2)
+        opt.step()
+        other.step()
+        assert all(torch.equal(x, y) for x, y in zip(p, b))
+    q = tensors([300], first, dev)
+    opt = P.AdamW(q, **HYPER)
+    set_grads(q, 1)
+    opt.step()
+    q[0].grad, q[0].data = None, q[0].data.to(then)
+    set_grads(q, 2)
+    check_step(opt, 2)
+
+
+def test_a_copy_serves_either_type_of_16_bits(dev):
+    p = tensors([300], torch.bfloat16, dev)
+    opt = P.AdamW(p, master_weights=True, **HYPER)
+    set_grads(p, 1)
+    opt.step()
+    p[0].grad, p[0].data = None, p[0].data.to(torch.float16)
+    set_grads(p, 2)
+    check_step(opt, 2)
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
