@@ -259,7 +259,7 @@ class AdamW(torch.optim.Optimizer):
             arena = self._arena(gi)
             work.append((gi, group, arena, self._gather(arena, group)))
         for gi, group, arena, todo in work:
-            with _lib.on_device(arena.device):
+            with _lib.on_device(arena.index):
                 self._step_group(gi, group, arena, todo)
         return loss
 
@@ -274,7 +274,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _step_group(self, gi, group, arena, todo):
         lr, (b1, b2) = group["lr"], group["betas"]
-        stream = _lib.stream(arena.device)
+        stream = _lib.stream(arena.index)
         wd, salt = float(group["weight_decay"]), self._salt(gi)
         lr_dev = lr if isinstance(lr, torch.Tensor) and self.capturable else None
         rates = (0.0 if lr_dev is not None else float(lr), float(b1), float(b2))
@@ -283,17 +283,21 @@ class AdamW(torch.optim.Optimizer):
                       _lib.ptr(arena.scalars), stream)
         for idx, dtype, ps, gs in todo:
             if idx is None:
-                self._touched(group["params"] + arena.written)
+                written = group["params"]
                 n, sizes, offsets = len(ps), arena.c_sizes, arena.c_offsets
             else:
-                self._touched([group["params"][i] for i in idx] + arena.written)
+                written = [group["params"][i] for i in idx]
                 n = len(idx)
                 sizes, offsets = (array("q", [x[i] for i in idx]) for x in (arena.sizes, arena.offsets))
             t = arena.steps[0 if idx is None else idx[0]] + (0 if self.capturable else 1)
             master = arena.master if dtype != torch.float32 else None
-            _lib.call("pin_adamw_step", *(x.buffer_info()[0] for x in (ps, gs, sizes, offsets)), n, _lib.TYPES[dtype],
-                      arena.bits, _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), _lib.ptr(master), arena.total,
-                      *rates, float(group["eps"]), wd, t, salt, _lib.ptr(arena.scalars), stream)
+            try:
+                _lib.call("pin_adamw_step", ps.buffer_info()[0], gs.buffer_info()[0], sizes.buffer_info()[0],
+                          offsets.buffer_info()[0], n, _lib.TYPES[dtype], arena.bits, _lib.ptr(arena.m), _lib.ptr(arena.v),
+                          _lib.ptr(arena.exps), _lib.ptr(master), arena.total, *rates, float(group["eps"]), wd, t, salt,
+                          _lib.ptr(arena.scalars), stream)
+            finally:   # (while the kernels run)
+                self._touched(written + arena.written)
             if self.capturable:
                 continue
             if idx is None:
@@ -316,9 +320,9 @@ class AdamW(torch.optim.Optimizer):
             return arena.m, arena.v
         m = torch.empty((arena.total,), dtype=torch.float32, device=arena.device)
         v = torch.empty_like(m)
-        with _lib.on_device(arena.device):
+        with _lib.on_device(arena.index):
             _lib.call("pin_adamw_moments", _lib.ptr(arena.m), _lib.ptr(arena.v), _lib.ptr(arena.exps), arena.total,
-                      _lib.ptr(m), _lib.ptr(v), _lib.stream(arena.device))
+                      _lib.ptr(m), _lib.ptr(v), _lib.stream(arena.index))
         return m, v
 
     def master(self, group=0):
