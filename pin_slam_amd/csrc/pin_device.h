@@ -1183,7 +1183,7 @@ __device__ __forceinline__ float mlp_sdf_packed(const MlpW& m, const float (&x)[
 
 // Two decodes sharing the weight reads (SDF and ReLU masks only, no gradient): the per-neighbour
 // training forward decodes neighbours j and j + 1 of a row together -- one LDS broadcast read of a
-// hidden-unit pair feeds both rows' packed FMAs, and the two chains are independent.  Each result
+// hidden-unit pair feeds both rows' FMAs, and the two chains are independent.  Each result
 // is mlp_sdf_packed<false>'s, bitwise (the same operations in the same order per row).
 __device__ __forceinline__ void mlp_sdf_packed_x2(const MlpW& m, const float (&xa)[kD], const float (&xb)[kD],
                                                   float& sa, float& sb, uint64_t& mka, uint64_t& mkb) {

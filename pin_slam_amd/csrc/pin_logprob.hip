@@ -127,7 +127,7 @@ __device__ __forceinline__ uint4 load_some(const typename T::type* p, int from, 
 
 // A row as aligned vectors of 16 bytes: vector u holds the classes u V - skip and on.  Its first and
 // last vector may be partly other rows'.  (Rows of an odd number of 16-bit classes, read at their own
-// alignment: 66 us for 2048 x 50021 bf16; in aligned vectors 43.)
+// alignment: 66 us for 2048 x 50021 bf16; in aligned vectors 44.)
 template <class T>
 struct Vectors {
     const typename T::type* base;
@@ -828,7 +828,8 @@ k_label_join_top(const typename T::type* __restrict__ logits, int classes, int64
 // Many long rows: a workgroup goes through a row alone, kPart vectors at a time, each thread with a running
 // maximum of its own (2^x is taken to it, and what it has summed is taken to a new one), so nothing waits
 // for the other threads before the row's end.
-// vectors of a part (of twice as many: 2048 x 50021 bf16 47 us instead of 44, 4096 x 131072 alike)
+// vectors of a part (of twice as many, inputs from memory: 2048 x 50021 bf16 50 us instead of 44, 4096 x 131072 207
+// instead of 190; in a training step, right behind a gradient of as many bytes, the former takes 62)
 constexpr int kPart = 256 * 4;
 static_assert((PIN_LABEL_CLASSES_MAX + 6) / 4 <= kSplits * 2 * kPart && (PIN_LABEL_CLASSES_MAX + 14) / 8 <= kSplits * kPart,
               "the longest row's parts");

@@ -19,9 +19,10 @@
 #include "pin_device.h"
 
 // Per-neighbour decoder (weighted_first False) of the fused grid kernel as one f32-MFMA GEMM per
-// neighbour slot (mlp_sdf_wave).  Off: measured 123 us vs 102 us on VALU for 262K queries -- the
-// f32 MFMA runs at the packed-f32 VALU rate on gfx950 and an 11-input hidden unit needs ~4 VALU
-// ops of post-processing (bias, ReLU, w2, mask) for ~5.5 packed FMAs saved.
+// neighbour slot (mlp_sdf_wave).  Off: measured 123 us vs 102 us on VALU for 262K queries, when the
+// VALU decoder still issued two FMAs at a time (packed f32, which the build has since given up) -- the
+// f32 MFMA runs at that rate on gfx950 and an 11-input hidden unit needs ~4 VALU ops of
+// post-processing (bias, ReLU, w2, mask) for the 11 FMAs saved.
 #ifndef PIN_MLP_MFMA
 #define PIN_MLP_MFMA 0
 #endif
