@@ -308,14 +308,24 @@ class AdamW(torch.optim.Optimizer):
                 arena.together = len(set(arena.steps)) == 1
         arena.held = None
 
+    def _seen(self, gi):
+        """What there is of a group's state; before its first step what that would find, which is not kept (a copy of the
+        parameters that is made here would miss what they are changed to before it)."""
+        group = self.param_groups[gi]
+        if gi % len(self.param_groups) in self._arenas and group["params"][0] in self.state:
+            return self._arena(gi)
+        for p in group["params"]:
+            _lib.require_device(p)
+        return _Arena(group, False)
+
     def offsets(self, group=0):
         """First element of each parameter of the group in the flat arrays."""
-        return list(self._arena(group).offsets)
+        return list(self._seen(group).offsets)
 
     def moments(self, group=0):
         """Both moments of a parameter group as flat float32 arrays (of 8-bit state: the values that
         its codes stand for; of 32-bit state: the state itself)."""
-        arena = self._arena(group)
+        arena = self._seen(group)
         if arena.bits == 32:
             return arena.m, arena.v
         m = torch.empty((arena.total,), dtype=torch.float32, device=arena.device)
@@ -327,7 +337,7 @@ class AdamW(torch.optim.Optimizer):
 
     def master(self, group=0):
         """The group's parameters in 32 bits as one flat array (None without master_weights)."""
-        return self._arena(group).master
+        return self._seen(group).master
 
     def state_dict(self):
         kept = dict(self.state)

@@ -987,6 +987,28 @@ def test_a_copy_serves_either_type_of_16_bits(dev):
     check_step(opt, 2)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_asking_before_the_first_step_keeps_nothing(dev, bits):
+    """moments(), master() and offsets() of a group that has not stepped: zeros, the parameters as they are, places; weights
+    that are loaded afterwards are those that the first step goes on from."""
+    a, b = tensors([300, 20], torch.bfloat16, dev), tensors([300, 20], torch.bfloat16, dev, 1)
+    opt = P.AdamW(a, state_bits=bits, master_weights=True, **HYPER)
+    ref = P.AdamW(b, state_bits=bits, master_weights=True, **HYPER)
+    assert opt.offsets() == [0, 512] and not any(bool(x.any()) for x in opt.moments())
+    assert torch.equal(opt.master()[:300], a[0].detach().float()) and opt.state_dict()["state"] == {}
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            p.copy_(q)
+    assert torch.equal(opt.master()[512:532], b[1].detach().float())
+    for t in (1, 2):
+        set_grads(a, t)
+        set_grads(b, t)
+        opt.step()
+        ref.step()
+        assert all(torch.equal(p, q) for p, q in zip([*a, *opt.moments(), opt.master()], [*b, *ref.moments(), ref.master()]))
+    assert opt.master() is opt.master() and opt.offsets() == [0, 512]
+
+
 def test_refusals(dev):
     ok = lambda: torch.nn.Parameter(torch.zeros(8, device=dev))   # noqa: E731
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
