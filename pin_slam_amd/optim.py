@@ -252,7 +252,8 @@ class AdamW(torch.optim.Optimizer):
                 lr = 0.0
             self._check_rates(group, lr)
             arena = self._arenas.get(gi)
-            if arena is not None and (arena.bits != group["state_bits"] or arena.master_weights != group["master_weights"]):
+            if arena is not None and (arena.bits != group["state_bits"] or (
+                    arena.master_weights != group["master_weights"] and (arena.master is not None) != _has_master(group))):
                 raise RuntimeError("AdamW: state_bits or master_weights changed after a group's first step")
             groups.append((gi, group))
         for gi, group in groups:

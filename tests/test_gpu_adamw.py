@@ -875,9 +875,10 @@ def test_rates_changed_later_are_checked_before_any_group_steps(dev, capturable)
     (params, opt), (others, ref) = build(), build()
     opt.step()
     ref.step()
-    for key, bad in (("lr", -1.0), ("lr", math.nan), ("betas", (0.9, 1.0)), ("betas", (-0.1, 0.9)), ("eps", -1e-3),
-                     ("weight_decay", math.inf), ("state_bits", 16), ("state_bits", 32), ("master_weights", True)):
-        group = opt.param_groups[1]
+    for gi, key, bad in ((1, "lr", -1.0), (1, "lr", math.nan), (1, "betas", (0.9, 1.0)), (1, "betas", (-0.1, 0.9)),
+                         (1, "eps", -1e-3), (1, "weight_decay", math.inf), (1, "state_bits", 16), (1, "state_bits", 32),
+                         (0, "master_weights", False)):
+        group = opt.param_groups[gi]
         kept, group[key] = group[key], bad
         versions = [p._version for p in params]
         with pytest.raises((ValueError, RuntimeError)):
@@ -886,6 +887,7 @@ def test_rates_changed_later_are_checked_before_any_group_steps(dev, capturable)
         assert [p._version for p in params] == versions
         assert all(torch.equal(p, q) for p, q in zip(params, others))
     assert [s["step"] for s in opt.state_dict()["state"].values()] == [1, 1, 1]
+    opt.param_groups[1]["master_weights"] = True   # of parameters in 32 bits: nothing changes
     opt.step()
     ref.step()
     assert all(torch.equal(p, q) for p, q in zip(params, others))
